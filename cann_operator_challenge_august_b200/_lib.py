@@ -8,6 +8,7 @@ library is missing or cannot be loaded, every entry point raises.
 from __future__ import annotations
 
 import ctypes
+import struct
 from pathlib import Path
 
 _PKG = Path(__file__).resolve().parent
@@ -24,7 +25,7 @@ STATUS_NAMES = {
 STATUS = {v: k for k, v in STATUS_NAMES.items()}
 
 # cgdrDataType
-DT_BF16, DT_FLOAT32, DT_FLOAT16, DT_INT64, DT_INT32 = 1, 2, 3, 4, 5
+DT_BF16, DT_FLOAT32, DT_FLOAT16, DT_INT64, DT_INT32, DT_FP8_E4M3 = 1, 2, 3, 4, 5, 6
 LAYOUT_HEAD_MAJOR, LAYOUT_TOKEN_MAJOR = 0, 1
 NUMERICS = {"reference": 0, "fp32_state": 1}
 
@@ -32,6 +33,9 @@ NOALLOC_SCRATCH_BYTES = 65536  # CGDR_NOALLOC_SCRATCH_BYTES
 
 DEVICE_WAIT_TIMEOUT = 0x1
 DEVICE_BAD_VARLEN = 0x2
+DEVICE_BAD_STATE_INDEX = 0x4
+
+RECURRENCE_CHUNK = 64  # CGDR_RECURRENCE_CHUNK
 
 # Every symbol declared in include/*.h, by header.
 EXPORTS_BY_HEADER = {
@@ -64,6 +68,17 @@ EXPORTS_BY_HEADER = {
         "cgdrGetGdrPath",
         "cgdrChunkGatedDeltaRule",
         "cgdrDestroyGdrExecutor",
+    ),
+    "cgdr_recurrence.h": (
+        "cgdrRecurrentGatedDeltaRule",
+        "cgdrGatedLinearRecurrence",
+        "cgdrGatedLinearRecurrenceBackward",
+        "cgdrGatedLinearRecurrenceStep",
+    ),
+    "cgdr_rms_norm.h": (
+        "cgdrRmsNorm",
+        "cgdrRmsNormBackwardGetWorkspaceSize",
+        "cgdrRmsNormBackward",
     ),
 }
 EXPORTS = tuple(sym for syms in EXPORTS_BY_HEADER.values() for sym in syms)
@@ -118,6 +133,19 @@ class CgdrFwdHPlan(ctypes.Structure):
 
     def as_dict(self) -> dict:
         return {name: getattr(self, name) for name, _ in self._fields_}
+
+
+# A cgdrTensor as bytes: struct.pack fills it in about a microsecond, a
+# ctypes.Structure field by field in several.  A bytes object passed as
+# char* lends its buffer for the length of the call.
+_VIEW = struct.Struct("@Pii8q8q")
+assert _VIEW.size == ctypes.sizeof(CgdrTensor)
+_ZEROS = tuple((0,) * (MAX_DIMS - n) for n in range(MAX_DIMS + 1))
+
+
+def view(data_ptr: int, dtype: int, shape, strides) -> bytes:
+    pad = _ZEROS[len(shape)]
+    return _VIEW.pack(data_ptr, dtype, len(shape), *shape, *pad, *strides, *pad)
 
 
 _lib = None
@@ -184,6 +212,17 @@ def load() -> ctypes.CDLL:
     lib.cgdrDestroyGdrExecutor.restype = None
     lib.cgdrPrepareChunkIndices.argtypes = [T, ctypes.c_int64, T, T, ctypes.c_void_p]
     lib.cgdrPrepareChunkIndices.restype = ctypes.c_int
+    # the one-call entries take their tensors as packed bytes (see view())
+    V, P = ctypes.c_char_p, ctypes.c_void_p
+    lib.cgdrRecurrentGatedDeltaRule.argtypes = [V] * 8 + [ctypes.c_float, V, P, P]
+    lib.cgdrGatedLinearRecurrence.argtypes = [V] * 7 + [P]
+    lib.cgdrGatedLinearRecurrenceBackward.argtypes = [V] * 10 + [P]
+    lib.cgdrGatedLinearRecurrenceStep.argtypes = [V] * 5 + [P, P]
+    lib.cgdrRmsNorm.argtypes = [V] * 4 + [ctypes.c_double, ctypes.c_int64] + [V] * 3 + [P]
+    lib.cgdrRmsNormBackwardGetWorkspaceSize.argtypes = [V, V, u64p]
+    lib.cgdrRmsNormBackward.argtypes = [V] * 3 + [ctypes.c_double] + [V] * 5 + [P, ctypes.c_uint64, P]
+    for name in EXPORTS_BY_HEADER["cgdr_recurrence.h"] + EXPORTS_BY_HEADER["cgdr_rms_norm.h"]:
+        getattr(lib, name).restype = ctypes.c_int
     lib.cgdrGetAbiVersion.argtypes = []
     lib.cgdrGetAbiVersion.restype = ctypes.c_int32
     _lib = lib

@@ -3,7 +3,7 @@
     python -m cann_operator_challenge_august_b200.build     # or build() from Python
 
 produces ``cann_operator_challenge_august_b200/libcgdr_fwd_h.so``: the C ABI
-of include/cgdr_fwd_h.h with the tensor-core and general kernels, and
+of include/*.h with all kernels, and
 ``runner/cgdr_fwd_h_case``: the golden-case runner (a plain C++ program over
 that C ABI).  nvcc cross-compiles without a GPU.
 """
@@ -19,7 +19,8 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 LIB = PKG / "libcgdr_fwd_h.so"
-SOURCES = [PKG / "csrc" / n for n in ("cgdr_fwd_h.cu", "cgdr_chunk_o.cu", "cgdr_wy.cu", "cgdr_gdr.cu", "host_util.cu")]
+SOURCES = [PKG / "csrc" / n for n in ("cgdr_fwd_h.cu", "cgdr_chunk_o.cu", "cgdr_wy.cu", "cgdr_gdr.cu",
+                                      "cgdr_recurrence.cu", "cgdr_rms_norm.cu", "host_util.cu")]
 RUNNER_SRC = PKG / "runner" / "cgdr_fwd_h_case.cpp"
 RUNNER = PKG / "runner" / "cgdr_fwd_h_case"
 HEADERS = sorted((PKG / "csrc").glob("*.cuh")) + sorted((ROOT / "include").glob("*.h"))
@@ -30,6 +31,7 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC,-O3",
     "-Xptxas", "-v",
     "--expt-relaxed-constexpr",
+    "--threads", "0",  # the sources side by side
     "-shared",
 ]
 
