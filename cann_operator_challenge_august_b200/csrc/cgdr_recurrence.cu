@@ -4,6 +4,7 @@
 
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 
 #include "../../include/cgdr_recurrence.h"
 #include "host_util.cuh"
@@ -68,10 +69,16 @@ cgdrStatus check_pool(const cgdrTensor* state, const cgdrTensor* idx, int64_t B,
     return CGDR_STATUS_SUCCESS;
 }
 
+cgdrStatus cuda_failed(const char* what, cudaError_t e)
+{
+    cudaGetLastError();
+    return fail(CGDR_STATUS_CUDA_ERROR, "%s: %s", what, cudaGetErrorString(e));
+}
+
 cgdrStatus launched(const char* what)
 {
     const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return fail(CGDR_STATUS_CUDA_ERROR, "%s: %s", what, cudaGetErrorString(e));
+    if (e != cudaSuccess) return cuda_failed(what, e);
     g_err[0] = '\0';
     return CGDR_STATUS_SUCCESS;
 }
@@ -143,6 +150,14 @@ cgdrStatus check_gate_types(const cgdrTensor* x, const cgdrTensor* g)
     return CGDR_STATUS_SUCCESS;
 }
 
+// The kernels step over 16 rows with 32-bit offsets.
+cgdrStatus check_row_stride(const cgdrTensor* t, const char* name)
+{
+    if (t->shape[1] > 1 && t->strides[1] >= (int64_t(1) << 25))
+        return fail(CGDR_STATUS_UNSUPPORTED, "%s's rows must be less than 2^25 elements apart", name);
+    return CGDR_STATUS_SUCCESS;
+}
+
 // Arguments that the forward and the backward pass share.
 cgdrStatus check_scan(const cgdrTensor* x, const cgdrTensor* g, const cgdrTensor* h0, const cgdrTensor* cu,
                       ScanParams* p)
@@ -166,9 +181,10 @@ cgdrStatus check_scan(const cgdrTensor* x, const cgdrTensor* g, const cgdrTensor
         N = cu->shape[0] - 1;
         p->cu = static_cast<const int64_t*>(cu->data);
     }
-    if (T >= (int64_t(1) << 31) || D >= (int64_t(1) << 31) || N >= (int64_t(1) << 16))
-        return fail(CGDR_STATUS_UNSUPPORTED, "T and D must fit in 31 bits and the sequences in 16");
+    if (T >= (int64_t(1) << 30) || D >= (int64_t(1) << 30) || N >= (int64_t(1) << 16))
+        return fail(CGDR_STATUS_UNSUPPORTED, "T and D must fit in 30 bits and the sequences in 16");
     if ((st = check_inner_contiguous(x, "x")) || (st = check_inner_contiguous(g, "g"))) return st;
+    if ((st = check_row_stride(x, "x")) || (st = check_row_stride(g, "g"))) return st;
     p->B = B; p->T = T; p->D = D; p->N = N;
     p->x = x->data; p->x_sb = x->strides[0]; p->x_st = x->strides[1];
     p->g = g->data; p->g_sb = g->strides[0]; p->g_st = g->strides[1];
@@ -190,7 +206,8 @@ cgdrStatus check_like(const cgdrTensor* t, int32_t dtype, const ScanParams& p, c
     if ((st = check_rank(t, 3, name))) return st;
     if (t->dtype != dtype) return fail(CGDR_STATUS_BAD_DTYPE, "%s has the wrong type", name);
     if (!shape_is(t, {p.B, p.T, p.D})) return fail(CGDR_STATUS_BAD_SHAPE, "%s must have shape [B, T, D]", name);
-    return check_inner_contiguous(t, name);
+    if ((st = check_inner_contiguous(t, name))) return st;
+    return check_row_stride(t, name);
 }
 
 cgdrStatus check_state(const cgdrTensor* t, const ScanParams& p, const char* name)
@@ -215,27 +232,109 @@ cgdrStatus check_chunks(const cgdrTensor* t, ScanParams* p)
     return CGDR_STATUS_SUCCESS;
 }
 
-struct LaunchForward {
-    const ScanParams& p;
+// CTAs of a cluster, which share a slab's tokens: doubled while all CTAs still
+// fit on the GPU at once (`resident` CTAs an SM) and have a chunk each.
+int32_t scan_cluster(const ScanParams& p, int64_t slabs, int64_t resident)
+{
+    const int64_t tiles = (p.T + kScanChunk - 1) / kScanChunk;
+    int32_t c = 1;
+    while (c < kScanMaxCluster && 2 * c <= tiles && 2 * c * slabs <= 148 * resident) c *= 2;
+    return c;
+}
+
+// Whether TMA can read the rows: base and strides are multiples of 16 bytes.
+bool tma_rows(const cgdrTensor* t)
+{
+    if (!present(t)) return true;
+    const int64_t v = 16 / bytes_of(t->dtype);
+    if (reinterpret_cast<uintptr_t>(t->data) % 16 != 0) return false;
+    for (int i = 0; i < 2; ++i)
+        if (t->shape[i] > 1 && (t->strides[i] % v != 0 || t->strides[i] <= 0)) return false;
+    return true;
+}
+
+cgdrStatus scan_map(const cgdrTensor* t, int V, CUtensorMap* map, const char* name)
+{
+    if (!present(t)) return CGDR_STATUS_SUCCESS;
+    const int64_t B = t->shape[0], T = t->shape[1], D = t->shape[2], v = 16 / bytes_of(t->dtype);
+    // a dimension of one element has no stride of its own; any multiple of 16 bytes serves
+    const int64_t row = T > 1 ? t->strides[1] : (D + v - 1) / v * v;
+    const int64_t batch = B > 1 ? t->strides[0] : T * row;
+    return make_rows_map(map, t->data, static_cast<int>(bytes_of(t->dtype)), D, T, row, B, batch, 32 * V, kScanSteps, name);
+}
+
+template <typename K>
+cudaError_t launch_scan(K kernel, ScanParams& p, const ScanMapsTma& maps, int V, int smem, int64_t resident,
+                        cudaStream_t stream)
+{
+    // the maps of 4 warps (twice, backwards) and 8 CTAs; 1 KB is the system's
+    const int64_t fit = 227 * 1024 / (smem + V * 8192 + 1024 + 128);
+    if (resident > fit) resident = fit;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    const int64_t slabs = (p.D + 32 * V - 1) / (32 * V);
+    p.cluster = scan_cluster(p, slabs * p.B, resident);
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(p.cluster);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3(static_cast<unsigned>(slabs * p.cluster), static_cast<unsigned>(p.B));
+    cfg.blockDim = dim3(kScanThreads);
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<const ScanParams>(p), maps);
+}
+
+// How the rows are read: two channels a lane by TMA; two by cp.async where
+// rows are no multiple of 16 bytes (of a lane's 4 or 8, then); one otherwise.
+enum class ScanPath { kTma, kPairs, kSingle };
+
+struct ScanLaunch {
+    ScanParams& p;
+    const ScanMapsTma& maps;
+    ScanPath path;
+    bool backward;
     cudaStream_t stream;
+    cudaError_t error = cudaSuccess;
+    template <typename TX, typename TG, int V, bool TMA>
+    void go()
+    {
+        error = backward ? launch_scan(scan_backward_kernel<TX, TG, V, TMA>, p, maps, V, scan_backward_smem<TX, TG, V>(),
+                                       3, stream)
+                         : launch_scan(scan_forward_kernel<TX, TG, V, TMA>, p, maps, V, scan_forward_smem<TX, TG, V>(),
+                                       4, stream);
+    }
     template <typename TX, typename TG>
     void operator()()
     {
-        const dim3 grid(static_cast<unsigned>((p.D + 127) / 128), static_cast<unsigned>(p.N));
-        scan_forward_kernel<TX, TG><<<grid, 128, 0, stream>>>(p);
+        if (path == ScanPath::kTma) go<TX, TG, 2, true>();
+        else if (path == ScanPath::kPairs) go<TX, TG, 2, false>();
+        else go<TX, TG, 1, false>();
     }
 };
 
-struct LaunchBackward {
-    const ScanParams& p;
-    cudaStream_t stream;
-    template <typename TX, typename TG>
-    void operator()()
-    {
-        const dim3 grid(static_cast<unsigned>((p.D + 127) / 128), static_cast<unsigned>(p.N));
-        scan_backward_kernel<TX, TG><<<grid, 128, 0, stream>>>(p);
-    }
-};
+cgdrStatus run_scan(ScanParams& p, const cgdrTensor* x, const cgdrTensor* g, const cgdrTensor* d_out,
+                    std::initializer_list<const cgdrTensor*> outs, bool backward, const char* what, void* stream)
+{
+    bool pairs = pieces_aligned(x, 2) && pieces_aligned(g, 2) && pieces_aligned(d_out, 2);
+    for (const cgdrTensor* t : outs) pairs = pairs && pieces_aligned(t, 2);
+    const bool tma = pairs && tma_rows(x) && tma_rows(g) && tma_rows(d_out);
+    ScanMapsTma maps;
+    memset(&maps, 0, sizeof(maps));
+    cgdrStatus st;
+    if (tma && ((st = scan_map(x, 2, &maps.x, "x")) || (st = scan_map(g, 2, &maps.g, "g")) ||
+                (st = scan_map(d_out, 2, &maps.d_out, "d_out"))))
+        return st;
+    ScanLaunch launch{p, maps, tma ? ScanPath::kTma : pairs ? ScanPath::kPairs : ScanPath::kSingle, backward,
+                      static_cast<cudaStream_t>(stream)};
+    with_types(x->dtype, g->dtype, launch);
+    if (launch.error != cudaSuccess) return cuda_failed(what, launch.error);
+    return launched(what);
+}
 
 struct LaunchStep {
     LinearStepParams& p;
@@ -356,8 +455,7 @@ cgdrStatus cgdrGatedLinearRecurrence(const cgdrTensor* x, const cgdrTensor* g, c
         p.ht = static_cast<float*>(final_state->data);
         p.ht_sn = final_state->strides[0];
     }
-    with_types(x->dtype, g->dtype, LaunchForward{p, static_cast<cudaStream_t>(stream)});
-    return launched("gated linear recurrence");
+    return run_scan(p, x, g, nullptr, {out}, false, "gated linear recurrence", stream);
 }
 
 cgdrStatus cgdrGatedLinearRecurrenceBackward(const cgdrTensor* x, const cgdrTensor* g,
@@ -390,8 +488,7 @@ cgdrStatus cgdrGatedLinearRecurrenceBackward(const cgdrTensor* x, const cgdrTens
         p.d_h0 = static_cast<float*>(d_initial_state->data);
         p.dh0_sn = d_initial_state->strides[0];
     }
-    with_types(x->dtype, g->dtype, LaunchBackward{p, static_cast<cudaStream_t>(stream)});
-    return launched("gated linear recurrence, backward");
+    return run_scan(p, x, g, d_out, {dx, dg}, true, "gated linear recurrence, backward", stream);
 }
 
 cgdrStatus cgdrGatedLinearRecurrenceStep(const cgdrTensor* x, const cgdrTensor* g, const cgdrTensor* state,

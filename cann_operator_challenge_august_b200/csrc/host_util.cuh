@@ -57,6 +57,12 @@ inline bool tma_aligned(const cgdrTensor* t)
     return true;
 }
 
+// A tensor map without swizzle over [b][rows][cols] elements of `elem_bytes`
+// (2 or 4; only moved, never computed with), in boxes of box_rows x box_cols
+// (one b).  Strides in elements.  Rows and columns past the end read as zero.
+cgdrStatus make_rows_map(CUtensorMap* map, const void* base, int elem_bytes, int64_t cols, int64_t rows, int64_t row_stride,
+                         int64_t batches, int64_t batch_stride, uint32_t box_cols, uint32_t box_rows, const char* name);
+
 // A bf16 tensor map with 128-byte swizzle (64- or 32-byte with swizzle_bytes = 64 or 32) over `rank` dims given innermost
 // first (sizes in elements, strides in elements for dims 1..rank-1).
 cgdrStatus make_map(CUtensorMap* map, void* base, int rank, const int64_t* size, const int64_t* stride,

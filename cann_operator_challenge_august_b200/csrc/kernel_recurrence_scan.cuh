@@ -1,14 +1,46 @@
 // The diagonal recurrence over whole sequences, forwards and backwards
 // (include/cgdr_recurrence.h).
+//
+// One cluster of CTAs walks along the tokens of one slab of 32 V channels, a
+// segment of 64 tokens a CTA at a time; a lane owns V channels, a warp 16
+// consecutive tokens of its CTA's 64.  Per segment:
+//   1. every warp runs its 16 steps from a zero state and keeps the factor
+//      A = prod exp(g) and the end state B, so that the true end state is
+//      A h_in + B;
+//   2. the CTA's warps join their (A, B) through shared memory, the CTAs
+//      theirs through distributed shared memory (every CTA tells all), and
+//      everyone folds the state that enters the next segment;
+//   3. every warp repeats its 16 steps from its true h_in and stores them.
+// x and g are read once and out is written once.  A warp brings its own 16
+// rows of the next segments into its own shared memory, by TMA where rows
+// allow it (16-byte multiples) and by cp.async otherwise, so the ring needs no
+// barrier between warps and the copies run on while the CTA joins.  Every sum
+// is taken in a fixed order, so the results are the same on every run.
+//
+// Backwards, the same with u_t = exp(g_{t+1}) dh_{t+1} folded from the right
+// (the factors A are the same), and with h_{t-1} recomputed from the state
+// that the forward pass saved before each 64 tokens.
+//
+// Sequences.  At a sequence's first token the running state is replaced by
+// its initial state, at its last token (backwards) u by d_final_state; a warp
+// that does so marks its B as independent of what enters (`cut`), rather than
+// relying on A = 0, so that NaN and infinities stay in their sequence.
 #pragma once
+
+#include <cuda.h>
 
 #include <cstdint>
 
+#include "ptx.cuh"
 #include "vec_io.cuh"
 
 namespace cgdr {
 
-constexpr int kScanChunk = 64;  // CGDR_RECURRENCE_CHUNK
+constexpr int kScanChunk = 64;    // CGDR_RECURRENCE_CHUNK: tokens of a CTA and segment
+constexpr int kScanWarps = 4;
+constexpr int kScanThreads = kScanWarps * 32;
+constexpr int kScanSteps = kScanChunk / kScanWarps;
+constexpr int kScanMaxCluster = 8;
 
 struct ScanParams {
     const void *x, *g, *d_out;
@@ -19,86 +51,828 @@ struct ScanParams {
     int64_t B, T, D, N;
     int64_t x_sb, x_st, g_sb, g_st, o_sb, o_st, do_sb, do_st, dx_sb, dx_st, dg_sb, dg_st;
     int64_t h0_sn, ht_sn, dht_sn, dh0_sn;
+    int32_t cluster;
 };
 
-struct ScanSeq {
-    int64_t b, begin, end, tail;  // tail: rows [end, tail) belong to no sequence
+// The warp's index in a register that the compiler knows to be uniform, so
+// that row addresses are formed once a warp.
+__device__ __forceinline__ int scan_warp() { return __shfl_sync(~0u, static_cast<int>(threadIdx.x / 32), 0); }
+
+// ---- sequences ------------------------------------------------------------------------
+
+struct ScanSpan {
+    int64_t first, last;  // tokens [first, last) belong to sequences
 };
 
-__device__ __forceinline__ int64_t scan_bound(const ScanParams& p, int64_t n)
+__device__ __forceinline__ ScanSpan scan_span(const ScanParams& p)
 {
-    const int64_t c = p.cu[n];
-    return c < 0 ? 0 : c > p.T ? p.T : c;
-}
-
-__device__ __forceinline__ ScanSeq scan_seq(const ScanParams& p, int64_t n)
-{
-    ScanSeq s;
-    s.b = p.cu ? 0 : n;
-    s.begin = p.cu ? scan_bound(p, n) : 0;
-    s.end = p.cu ? scan_bound(p, n + 1) : p.T;
-    s.tail = n == p.N - 1 ? p.T : s.end;
+    ScanSpan s{0, p.T};
+    if (p.cu) {
+        s.first = p.cu[0];
+        const int64_t last = p.cu[p.N];
+        s.last = last < p.T ? last : p.T;
+    }
     return s;
 }
 
-// One thread: one channel of one sequence, token by token.
-template <typename TX, typename TG>
-__global__ void __launch_bounds__(128) scan_forward_kernel(const ScanParams p)
+// Bit i: a sequence begins or ends before token t + i, 0 <= i <= 16.
+__device__ __forceinline__ uint32_t scan_borders(const ScanParams& p, int64_t t)
 {
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x, n = blockIdx.y;
-    if (c >= p.D) return;
-    const ScanSeq s = scan_seq(p, n);
-    const TX* const x = static_cast<const TX*>(p.x) + s.b * p.x_sb + c;
-    const TG* const g = static_cast<const TG*>(p.g) + s.b * p.g_sb + c;
-    TX* const o = static_cast<TX*>(p.out) + s.b * p.o_sb + c;
-    const int64_t nc = (p.T + kScanChunk - 1) / kScanChunk;
-    float h = p.h0 ? p.h0[n * p.h0_sn + c] : 0.0f;
-    for (int64_t t = s.begin; t < s.end; ++t) {
-        if (p.chunk && t % kScanChunk == 0) p.chunk[(s.b * nc + t / kScanChunk) * p.D + c] = h;
-        h = fmaf(expf(to_f32(g[t * p.g_st])), h, to_f32(x[t * p.x_st]));
-        o[t * p.o_st] = from_f32<TX>(h);
+    if (!p.cu) {
+        const int64_t to_end = p.T - t;
+        return (t == 0 ? 1u : 0u) | (to_end >= 0 && to_end <= kScanSteps ? 1u << to_end : 0u);
     }
-    if (p.ht) p.ht[n * p.ht_sn + c] = h;
-    for (int64_t t = s.end; t < s.tail; ++t) o[t * p.o_st] = from_f32<TX>(0.0f);
+    uint32_t bits = 0;
+    for (int64_t i = threadIdx.x % 32; i <= p.N; i += 32) {
+        const int64_t d = p.cu[i] - t;
+        if (d >= 0 && d <= kScanSteps) bits |= 1u << d;
+    }
+    return __reduce_or_sync(~0u, bits);
 }
 
-template <typename TX, typename TG>
-__global__ void __launch_bounds__(128) scan_backward_kernel(const ScanParams p)
+// The sequence of token t: the last one that begins at or before it.
+__device__ __forceinline__ int64_t scan_sequence(const ScanParams& p, int64_t b, int64_t t)
 {
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * 128 + threadIdx.x, n = blockIdx.y;
-    if (c >= p.D) return;
-    const ScanSeq s = scan_seq(p, n);
-    const TX* const x = static_cast<const TX*>(p.x) + s.b * p.x_sb + c;
-    const TG* const g = static_cast<const TG*>(p.g) + s.b * p.g_sb + c;
-    const TX* const d_out = p.d_out ? static_cast<const TX*>(p.d_out) + s.b * p.do_sb + c : nullptr;
-    TX* const dx = p.dx ? static_cast<TX*>(p.dx) + s.b * p.dx_sb + c : nullptr;
-    TG* const dg = p.dg ? static_cast<TG*>(p.dg) + s.b * p.dg_sb + c : nullptr;
-    const int64_t nc = (p.T + kScanChunk - 1) / kScanChunk;
-    for (int64_t t = s.end; t < s.tail; ++t) {
-        if (dx) dx[t * p.dx_st] = from_f32<TX>(0.0f);
-        if (dg) dg[t * p.dg_st] = from_f32<TG>(0.0f);
+    if (!p.cu) return b;
+    unsigned before = 0;
+    for (int64_t i = threadIdx.x % 32; i <= p.N; i += 32) before += p.cu[i] <= t;
+    const int64_t n = static_cast<int64_t>(__reduce_add_sync(~0u, before)) - 1;
+    return n < 0 ? 0 : n < p.N ? n : p.N - 1;
+}
+
+template <int V>
+__device__ __forceinline__ void scan_load_state(const float* base, int64_t stride, int64_t n, int64_t c, bool mine,
+                                                float* out)
+{
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = base && mine ? base[n * stride + c + i] : 0.0f;
+}
+
+template <int V>
+__device__ __forceinline__ void scan_store_state(float* base, int64_t stride, int64_t n, int64_t c, bool mine,
+                                                 const float* v)
+{
+    if (!base || !mine) return;
+#pragma unroll
+    for (int i = 0; i < V; ++i) base[n * stride + c + i] = v[i];
+}
+
+// States of empty sequences pass through (`to` from `from`).
+template <int V>
+__device__ __forceinline__ void scan_empty_sequences(const ScanParams& p, const float* from, int64_t from_s, float* to,
+                                                     int64_t to_s, int64_t c, bool mine)
+{
+    if (!p.cu || !to) return;
+    for (int64_t n = threadIdx.x / 32; n < p.N; n += kScanWarps) {
+        if (p.cu[n + 1] > p.cu[n]) continue;
+        float h[V];
+        scan_load_state<V>(from, from_s, n, c, mine, h);
+        scan_store_state<V>(to, to_s, n, c, mine, h);
     }
-    float u = p.d_ht ? p.d_ht[n * p.dht_sn + c] : 0.0f;  // exp(g_{t+1}) dh_{t+1}
-    float before[kScanChunk];                            // h_{t-1}
-    for (int64_t stop = s.end; stop > s.begin;) {
-        const int64_t floor = (stop - 1) / kScanChunk * kScanChunk;
-        const int64_t first = floor > s.begin ? floor : s.begin;
-        float h = first > s.begin ? p.chunk[(s.b * nc + first / kScanChunk) * p.D + c]
-                  : p.h0          ? p.h0[n * p.h0_sn + c]
-                                  : 0.0f;
-        for (int64_t t = first; t < stop; ++t) {
-            before[t - first] = h;
-            h = fmaf(expf(to_f32(g[t * p.g_st])), h, to_f32(x[t * p.x_st]));
-        }
-        for (int64_t t = stop - 1; t >= first; --t) {
-            const float dh = u + (d_out ? to_f32(d_out[t * p.do_st]) : 0.0f);
-            u = dh * expf(to_f32(g[t * p.g_st]));
-            if (dx) dx[t * p.dx_st] = from_f32<TX>(dh);
-            if (dg) dg[t * p.dg_st] = from_f32<TG>(u * before[t - first]);
-        }
-        stop = first;
+}
+
+// ---- arithmetic on a lane's V channels, two at a time where V is even -----------------------
+
+__device__ __forceinline__ uint64_t f32x2(float a, float b)
+{
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void f32x2_split(uint64_t v, float& a, float& b)
+{
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+
+template <int V>
+__device__ __forceinline__ void vec_fma(const float* a, const float* b, const float* c, float* to)
+{
+    if constexpr (V == 2) {
+        uint64_t r;
+        asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(f32x2(a[0], a[1])), "l"(f32x2(b[0], b[1])), "l"(f32x2(c[0], c[1])));
+        f32x2_split(r, to[0], to[1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) to[i] = fmaf(a[i], b[i], c[i]);
     }
-    if (p.d_h0) p.d_h0[n * p.dh0_sn + c] = u;
+}
+template <int V>
+__device__ __forceinline__ void vec_mul(const float* a, const float* b, float* to)
+{
+    if constexpr (V == 2) {
+        uint64_t r;
+        asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f32x2(a[0], a[1])), "l"(f32x2(b[0], b[1])));
+        f32x2_split(r, to[0], to[1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) to[i] = a[i] * b[i];
+    }
+}
+template <int V>
+__device__ __forceinline__ void vec_add(const float* a, const float* b, float* to)
+{
+    if constexpr (V == 2) {
+        uint64_t r;
+        asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f32x2(a[0], a[1])), "l"(f32x2(b[0], b[1])));
+        f32x2_split(r, to[0], to[1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) to[i] = a[i] + b[i];
+    }
+}
+template <typename T, int V>
+__device__ __forceinline__ void vec_f32(const Pack<T, V>& p, float* to)
+{
+#pragma unroll
+    for (int i = 0; i < V; ++i) to[i] = to_f32(p.e[i]);
+}
+// exp(g): by the hardware's exponential (within 2 ulp; the argument's own
+// rounding adds |g| half-ulps); results below 2^-126 are 0.
+template <typename T, int V>
+__device__ __forceinline__ void vec_exp(const Pack<T, V>& g, float* to)
+{
+    float x[V];
+    vec_f32<T, V>(g, x);
+    if constexpr (V == 2) {
+        const float log2e[2] = {1.4426950408889634f, 1.4426950408889634f};
+        vec_mul<V>(x, log2e, x);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[i] *= 1.4426950408889634f;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(to[i]) : "f"(x[i]));
+}
+
+// ---- the ring: each warp's own 16 rows -------------------------------------------------------
+
+// Rows of 32 V channels of one tensor, and how a warp brings 16 of them in.
+template <typename T, int V, bool TMA>
+struct ScanRows {
+    static constexpr int kLane = sizeof(T) * V;
+    static constexpr int kBytes = kLane * 32 * kScanSteps;  // of a warp and stage
+
+    // Rows t .. t + 16 of the slab to `to`.  By TMA: one lane calls, rows past
+    // the tensor's end are zero, all bytes count on `full`.  By cp.async: all
+    // lanes call, each copies what it will read; rows past `end` stay as they
+    // are.  `base`: the slab's first channel at token 0.
+    static __device__ __forceinline__ void fetch_tma(const CUtensorMap* map, int slab, int t, int b, uint64_t* full,
+                                                     uint8_t* to)
+    {
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+            " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(to)),
+            "l"(reinterpret_cast<uint64_t>(map)), "r"(slab), "r"(t), "r"(b), "r"(smem_u32(full))
+            : "memory");
+    }
+    static __device__ __forceinline__ void fetch(const T* base, int64_t stride, int64_t t, int64_t end, uint8_t* to)
+    {
+        const int lane = threadIdx.x % 32;
+        const uint8_t* const row = reinterpret_cast<const uint8_t*>(base + t * stride) + lane * kLane;
+        const uint32_t step = static_cast<uint32_t>(stride) * sizeof(T);  // below 2^27: checked by the host
+        const int count = end - t >= kScanSteps ? kScanSteps : end > t ? static_cast<int>(end - t) : 0;
+        to += lane * kLane;
+        if constexpr (kLane >= 4) {
+            const uint32_t at = smem_u32(to);
+            if (count == kScanSteps) {
+#pragma unroll
+                for (int l = 0; l < kScanSteps; ++l) copy(at + l * 32 * kLane, row + l * step);
+            } else {
+                for (int l = 0; l < count; ++l) copy(at + l * 32 * kLane, row + l * step);
+            }
+        } else {  // two bytes: too small for cp.async
+            T e[kScanSteps];
+#pragma unroll
+            for (int l = 0; l < kScanSteps; ++l)
+                if (l < count) e[l] = *reinterpret_cast<const T*>(row + l * step);
+#pragma unroll
+            for (int l = 0; l < kScanSteps; ++l)
+                if (l < count) *reinterpret_cast<T*>(to + l * 32 * kLane) = e[l];
+        }
+    }
+    static __device__ __forceinline__ void copy(uint32_t to, const uint8_t* from)
+    {
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(kLane) : "memory");
+    }
+    static __device__ __forceinline__ Pack<T, V> get(const uint8_t* stage, int l)
+    {
+        return load_pack<T, V, true>(reinterpret_cast<const T*>(stage + (l * 32 + threadIdx.x % 32) * kLane));
+    }
+};
+
+__device__ __forceinline__ void scan_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+template <int PENDING>
+__device__ __forceinline__ void scan_wait()
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
+
+constexpr uint64_t kScanWaitNs = 2000000000ull;
+
+// Waits for a barrier's phase, two seconds at most.  A wait that runs out is
+// remembered: the CTA waits no more and its states become NaN.
+__device__ __forceinline__ bool scan_await(uint64_t* bar, uint32_t parity, volatile bool* lost)
+{
+    const uint32_t addr = smem_u32(bar);
+    if (mbar_try_wait(addr, parity)) return true;
+    const uint64_t since = global_timer_ns();
+    while (!*lost) {
+#pragma unroll 1
+        for (int i = 0; i < 32; ++i)
+            if (mbar_try_wait(addr, parity)) return true;
+        if (global_timer_ns() - since > kScanWaitNs) *lost = true;
+    }
+    return false;
+}
+
+// This lane's elements of row `l` behind `base` (token t of the slab).
+template <typename T, int V>
+__device__ __forceinline__ void scan_store(T* base, int64_t stride, int64_t t, int l, const float* v)
+{
+    const uint32_t step = static_cast<uint32_t>(stride) * sizeof(T);
+    uint8_t* const row = reinterpret_cast<uint8_t*>(base + t * stride) + threadIdx.x % 32 * (sizeof(T) * V);
+    store_pack<T, V, true>(reinterpret_cast<T*>(row + l * step), v);
+}
+
+// ---- joining ------------------------------------------------------------------------------
+
+// What a warp or a CTA does to the value that enters it: cut ? b : a v + b.
+template <int V>
+struct ScanMap {
+    float a[V], b[V];
+    bool cut;
+    __device__ __forceinline__ void clear()
+    {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            a[i] = 1.0f;
+            b[i] = 0.0f;
+        }
+        cut = false;
+    }
+    __device__ __forceinline__ void cut_to_zero()
+    {
+#pragma unroll
+        for (int i = 0; i < V; ++i) b[i] = 0.0f;
+        cut = true;
+    }
+    __device__ __forceinline__ void apply(float* v) const
+    {
+        float r[V];
+        vec_fma<V>(a, v, b, r);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = cut ? b[i] : r[i];
+    }
+    // this, then `next`
+    __device__ __forceinline__ void then(const ScanMap& next)
+    {
+        next.apply(b);
+        cut |= next.cut;
+        vec_mul<V>(a, next.a, a);
+    }
+};
+
+// A lane's part of a map on its way through shared memory: one access of 8 V
+// bytes.  A factor is never negative, so a[0] = -1 tells that the map cuts.
+template <int V>
+struct alignas(8 * V) ScanSlot {
+    float a[V], b[V];
+    __device__ __forceinline__ explicit ScanSlot(const ScanMap<V>& m)
+    {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            a[i] = m.a[i];
+            b[i] = m.b[i];
+        }
+        if (m.cut) a[0] = -1.0f;
+    }
+    __device__ __forceinline__ operator ScanMap<V>() const
+    {
+        ScanMap<V> m;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            m.a[i] = a[i];
+            m.b[i] = b[i];
+        }
+        m.cut = a[0] < 0.0f;
+        return m;
+    }
+};
+
+// Maps of K partners for 32 lanes in shared memory, twice: a segment's writes
+// never meet reads of the segment before, which lie a barrier behind.
+template <int V, int K>
+struct ScanMaps {
+    alignas(16) uint8_t bytes[2][K][32 * sizeof(ScanSlot<V>)];
+    __device__ __forceinline__ ScanSlot<V>* at(int turn, int k)
+    {
+        return reinterpret_cast<ScanSlot<V>*>(bytes[turn][k]) + threadIdx.x % 32;
+    }
+};
+
+// The same for the CTAs of a cluster, with a barrier for each turn that counts
+// the bytes which the CTAs (this one too) send.
+template <int V>
+struct ScanCluster {
+    ScanMaps<V, kScanMaxCluster> maps;
+    alignas(8) uint64_t full[2];
+};
+
+__device__ __forceinline__ void scan_cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+}
+
+template <int V>
+__device__ __forceinline__ void scan_cluster_open(ScanCluster<V>& s)
+{
+    if (threadIdx.x == 0) {
+        mbar_init(&s.full[0], 1);
+        mbar_init(&s.full[1], 1);
+        fence_mbarrier_init();
+    }
+    scan_cluster_sync();  // no CTA sends before all have started and set up their barriers
+}
+
+// Lane's slot -> CTA `rank`'s copy of it; the bytes count on that CTA's barrier.
+template <int V>
+__device__ __forceinline__ void scan_send(ScanSlot<V>* to, uint64_t* bar, int rank, const ScanSlot<V>& v)
+{
+    uint32_t at, b;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(to)), "r"(rank));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(smem_u32(bar)), "r"(rank));
+    if constexpr (V == 2)
+        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(at),
+                     "f"(v.a[0]), "f"(v.a[1]), "f"(v.b[0]), "f"(v.b[1]), "r"(b)
+                     : "memory");
+    else
+        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(at),
+                     "f"(v.a[0]), "f"(v.b[0]), "r"(b)
+                     : "memory");
+}
+
+// Folds `value` (what enters segment k) through the CTAs of the cluster in
+// their order, or the reverse, and returns what enters this CTA; afterwards
+// `value` is what leaves the segment.  `mine` is the whole CTA's map.  A map's
+// slots are written again two segments later, by CTAs that have this CTA's
+// map of the segment between, which it sends when all its warps have read.
+template <int V, bool REVERSE>
+__device__ __forceinline__ void scan_join_cluster(ScanCluster<V>& s, int k, int ctas, int rank, const ScanMap<V>& mine,
+                                                  float* value, float* enters, volatile bool* lost)
+{
+    const int turn = k & 1;
+    if (threadIdx.x == 0) mbar_arrive_expect_tx(&s.full[turn], ctas * 32 * sizeof(ScanSlot<V>));
+    const ScanSlot<V> slot(mine);
+    for (int to = scan_warp(); to < ctas; to += kScanWarps)
+        scan_send<V>(s.maps.at(turn, rank), &s.full[turn], to, slot);
+    const bool there = scan_await(&s.full[turn], k >> 1 & 1, lost);
+#pragma unroll 2
+    for (int n = 0; n < ctas; ++n) {
+        const int r = REVERSE ? ctas - 1 - n : n;
+        if (r == rank) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) enters[i] = value[i];
+        }
+        ScanMap<V>(*s.maps.at(turn, r)).apply(value);
+    }
+    if (!there) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) value[i] = enters[i] = __int_as_float(0x7fffffff);
+    }
+}
+
+// From the warps' maps of a CTA in their order, or the reverse: what all do,
+// and what those before this warp do.
+template <int V, bool REVERSE>
+__device__ __forceinline__ void scan_join_warps(ScanMaps<V, kScanWarps>& maps, int turn, int warp, ScanMap<V>& before,
+                                                ScanMap<V>& all)
+{
+    ScanMap<V> m[kScanWarps];
+#pragma unroll
+    for (int w = 0; w < kScanWarps; ++w) m[w] = *maps.at(turn, REVERSE ? kScanWarps - 1 - w : w);
+    all.clear();
+#pragma unroll
+    for (int w = 0; w < kScanWarps; ++w) {
+        if (w == (REVERSE ? kScanWarps - 1 - warp : warp)) before = all;
+        all.then(m[w]);
+    }
+}
+
+// ---- forwards -------------------------------------------------------------------------------
+
+constexpr int kScanStages = 2;
+
+// A CTA's copies: kScanStages x kScanWarps pieces of NT tensors' rows.
+template <int NT, bool TMA>
+struct ScanFlight {
+    alignas(8) uint64_t full[TMA ? kScanStages : 1][kScanWarps];
+    bool lost;  // a wait ran out
+    __device__ __forceinline__ void open()
+    {
+        if (threadIdx.x == 0) {
+            lost = false;
+            if constexpr (TMA) {
+#pragma unroll
+                for (int i = 0; i < kScanStages * kScanWarps; ++i) mbar_init(&full[0][0] + i, 1);
+                fence_mbarrier_init();
+            }
+        }
+        __syncthreads();
+    }
+    // Waits for the warp's piece k.
+    __device__ __forceinline__ bool wait(int warp, int k)
+    {
+        if constexpr (TMA) return scan_await(&full[k % kScanStages][warp], k / kScanStages & 1, &lost);
+        scan_wait<kScanStages - 1>();
+        return true;
+    }
+};
+
+struct ScanMapsTma {
+    CUtensorMap x, g, d_out;  // [B, T, D] in boxes of 16 rows and 32 V channels
+};
+
+template <typename TX, typename TG, int V>
+constexpr int scan_forward_smem()
+{
+    return kScanStages * kScanWarps * (ScanRows<TX, V, true>::kBytes + ScanRows<TG, V, true>::kBytes);
+}
+
+template <typename TX, typename TG, int V, bool TMA>
+__global__ void __launch_bounds__(kScanThreads, 4)
+    scan_forward_kernel(const ScanParams p, const __grid_constant__ ScanMapsTma maps)
+{
+    using RX = ScanRows<TX, V, TMA>;
+    using RG = ScanRows<TG, V, TMA>;
+    constexpr int kPiece = RX::kBytes + RG::kBytes;
+    extern __shared__ __align__(128) uint8_t ring[];
+    __shared__ ScanMaps<V, kScanWarps> warps;
+    __shared__ ScanCluster<V> ctas;
+    __shared__ ScanFlight<2, TMA> flight;
+
+    const int warp = scan_warp(), lane = threadIdx.x % 32;
+    const int rank = blockIdx.x % p.cluster;
+    const int64_t slab = static_cast<int64_t>(blockIdx.x / p.cluster) * 32 * V, c = slab + lane * V, b = blockIdx.y;
+    const bool mine = c < p.D;
+    const int64_t tiles = (p.T + kScanChunk - 1) / kScanChunk;
+    const int segments = static_cast<int>((tiles + p.cluster - 1) / p.cluster);
+    const ScanSpan span = scan_span(p);
+    TX* const out = static_cast<TX*>(p.out) + b * p.o_sb + slab;
+
+    auto first_token = [&](int seg) {
+        return (static_cast<int64_t>(seg) * p.cluster + rank) * kScanChunk + warp * kScanSteps;
+    };
+    auto piece = [&](int seg) { return ring + (seg % kScanStages * kScanWarps + warp) * kPiece; };
+    auto fetch = [&](int seg) {
+        uint8_t* const to = piece(seg);
+        if constexpr (TMA) {
+            if (seg < segments) {
+                __syncwarp();  // all lanes have read what the piece held
+                if (lane == 0) {
+                    uint64_t* const full = &flight.full[seg % kScanStages][warp];
+                    const int t = static_cast<int>(first_token(seg));
+                    mbar_arrive_expect_tx(full, kPiece);
+                    RX::fetch_tma(&maps.x, static_cast<int>(slab), t, static_cast<int>(b), full, to);
+                    RG::fetch_tma(&maps.g, static_cast<int>(slab), t, static_cast<int>(b), full, to + RX::kBytes);
+                }
+            }
+        } else {
+            if (seg < segments && mine) {
+                const int64_t t = first_token(seg);
+                RX::fetch(static_cast<const TX*>(p.x) + b * p.x_sb + slab, p.x_st, t, p.T, to);
+                RG::fetch(static_cast<const TG*>(p.g) + b * p.g_sb + slab, p.g_st, t, p.T, to + RX::kBytes);
+            }
+            scan_commit();
+        }
+    };
+    flight.open();
+#pragma unroll
+    for (int s = 0; s < kScanStages; ++s) fetch(s);
+    if (p.cluster > 1) scan_cluster_open(ctas);
+    if (rank == 0) scan_empty_sequences<V>(p, p.h0, p.h0_sn, p.ht, p.ht_sn, c, mine);
+
+    float state[V];  // what enters the segment
+#pragma unroll
+    for (int i = 0; i < V; ++i) state[i] = 0.0f;
+
+    for (int seg = 0; seg < segments; ++seg) {
+        const int turn = seg & 1;
+        const int64_t t = first_token(seg);
+        const uint32_t borders = scan_borders(p, t);
+        // nothing begins or ends in these steps, and all of them are a sequence's
+        const bool plain = borders == 0 && t >= span.first && t + kScanSteps <= span.last;
+        const bool there = flight.wait(warp, seg);
+        const uint8_t *const px = piece(seg), *const pg = px + RX::kBytes;
+
+        float a[kScanSteps][V], x[kScanSteps][V];
+        ScanMap<V> m;
+        m.clear();
+        if (plain) {
+#pragma unroll
+            for (int l = 0; l < kScanSteps; ++l) {
+                vec_f32<TX, V>(RX::get(px, l), x[l]);
+                vec_exp<TG, V>(RG::get(pg, l), a[l]);
+                vec_mul<V>(m.a, a[l], m.a);
+                vec_fma<V>(a[l], m.b, x[l], m.b);
+            }
+            fetch(seg + kScanStages);
+        } else {
+#pragma unroll 1
+            for (int l = 0; l < kScanSteps; ++l) {
+                const int64_t at = t + l;
+                if (at < span.first || at >= span.last) {  // no sequence's, or no token: the state is 0
+                    m.cut_to_zero();
+                    continue;
+                }
+                if (borders >> l & 1) {
+                    scan_load_state<V>(p.h0, p.h0_sn, scan_sequence(p, b, at), c, mine, m.b);
+                    m.cut = true;
+                }
+                vec_f32<TX, V>(RX::get(px, l), x[0]);
+                vec_exp<TG, V>(RG::get(pg, l), a[0]);
+                vec_mul<V>(m.a, a[0], m.a);
+                vec_fma<V>(a[0], m.b, x[0], m.b);
+            }
+        }
+        if (!there) m.b[0] = __int_as_float(0x7fffffff);
+
+        *warps.at(turn, warp) = ScanSlot<V>(m);
+        __syncthreads();
+        ScanMap<V> before, all;
+        scan_join_warps<V, false>(warps, turn, warp, before, all);
+        float h[V];
+        if (p.cluster == 1) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) h[i] = state[i];
+            all.apply(state);
+        } else {
+            scan_join_cluster<V, false>(ctas, seg, p.cluster, rank, all, state, h, &flight.lost);
+        }
+        before.apply(h);
+
+        if (p.chunk && warp == 0 && mine && t < p.T)
+            scan_store_state<V>(p.chunk, p.D, b * tiles + t / kScanChunk, c, mine, h);
+        if (plain) {
+#pragma unroll
+            for (int l = 0; l < kScanSteps; ++l) {
+                vec_fma<V>(a[l], h, x[l], h);
+                if (mine) scan_store<TX, V>(out, p.o_st, t, l, h);
+            }
+        } else {
+#pragma unroll 1
+            for (int l = 0; l < kScanSteps && t + l < p.T; ++l) {
+                const int64_t at = t + l;
+                if (at < span.first || at >= span.last) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) h[i] = 0.0f;
+                } else {
+                    if (borders >> l & 1) scan_load_state<V>(p.h0, p.h0_sn, scan_sequence(p, b, at), c, mine, h);
+                    vec_f32<TX, V>(RX::get(px, l), x[0]);
+                    vec_exp<TG, V>(RG::get(pg, l), a[0]);
+                    vec_fma<V>(a[0], h, x[0], h);
+                    if (p.ht && (borders >> (l + 1) & 1))
+                        scan_store_state<V>(p.ht, p.ht_sn, scan_sequence(p, b, at), c, mine, h);
+                }
+                if (mine) scan_store<TX, V>(out, p.o_st, t, l, h);
+            }
+            fetch(seg + kScanStages);
+        }
+    }
+    if (p.cluster > 1) scan_cluster_sync();  // none leaves while another may still send to it
+}
+
+// ---- backwards --------------------------------------------------------------------------------
+
+template <typename TX, typename TG, int V>
+constexpr int scan_backward_smem()
+{
+    return kScanStages * kScanWarps * (2 * ScanRows<TX, V, true>::kBytes + ScanRows<TG, V, true>::kBytes);
+}
+
+template <typename TX, typename TG, int V, bool TMA>
+__global__ void __launch_bounds__(kScanThreads, 3)
+    scan_backward_kernel(const ScanParams p, const __grid_constant__ ScanMapsTma maps)
+{
+    using RX = ScanRows<TX, V, TMA>;
+    using RG = ScanRows<TG, V, TMA>;
+    constexpr int kPiece = 2 * RX::kBytes + RG::kBytes;
+    extern __shared__ __align__(128) uint8_t ring[];
+    __shared__ ScanMaps<V, kScanWarps> warps_h, warps_u;
+    __shared__ ScanCluster<V> ctas;
+    __shared__ ScanFlight<3, TMA> flight;
+
+    const int warp = scan_warp(), lane = threadIdx.x % 32;
+    const int rank = blockIdx.x % p.cluster;
+    const int64_t slab = static_cast<int64_t>(blockIdx.x / p.cluster) * 32 * V, c = slab + lane * V, b = blockIdx.y;
+    const bool mine = c < p.D;
+    const int64_t tiles = (p.T + kScanChunk - 1) / kScanChunk;
+    const int segments = static_cast<int>((tiles + p.cluster - 1) / p.cluster);
+    const ScanSpan span = scan_span(p);
+    TX* const dx = p.dx ? static_cast<TX*>(p.dx) + b * p.dx_sb + slab : nullptr;
+    TG* const dg = p.dg ? static_cast<TG*>(p.dg) + b * p.dg_sb + slab : nullptr;
+
+    // segments run from the last to the first: turn k is segment segments - 1 - k
+    auto first_token = [&](int k) {
+        return (static_cast<int64_t>(segments - 1 - k) * p.cluster + rank) * kScanChunk + warp * kScanSteps;
+    };
+    auto piece = [&](int k) { return ring + (k % kScanStages * kScanWarps + warp) * kPiece; };
+    auto fetch = [&](int k) {
+        uint8_t* const to = piece(k);
+        if constexpr (TMA) {
+            if (k < segments) {
+                __syncwarp();
+                if (lane == 0) {
+                    uint64_t* const full = &flight.full[k % kScanStages][warp];
+                    const int t = static_cast<int>(first_token(k));
+                    mbar_arrive_expect_tx(full, p.d_out ? kPiece : kPiece - RX::kBytes);
+                    RX::fetch_tma(&maps.x, static_cast<int>(slab), t, static_cast<int>(b), full, to);
+                    RG::fetch_tma(&maps.g, static_cast<int>(slab), t, static_cast<int>(b), full, to + RX::kBytes);
+                    if (p.d_out)
+                        RX::fetch_tma(&maps.d_out, static_cast<int>(slab), t, static_cast<int>(b), full,
+                                      to + RX::kBytes + RG::kBytes);
+                }
+            }
+        } else {
+            if (k < segments && mine) {
+                const int64_t t = first_token(k);
+                RX::fetch(static_cast<const TX*>(p.x) + b * p.x_sb + slab, p.x_st, t, p.T, to);
+                RG::fetch(static_cast<const TG*>(p.g) + b * p.g_sb + slab, p.g_st, t, p.T, to + RX::kBytes);
+                if (p.d_out)
+                    RX::fetch(static_cast<const TX*>(p.d_out) + b * p.do_sb + slab, p.do_st, t, p.T,
+                              to + RX::kBytes + RG::kBytes);
+            }
+            scan_commit();
+        }
+    };
+    flight.open();
+#pragma unroll
+    for (int s = 0; s < kScanStages; ++s) fetch(s);
+    if (p.cluster > 1) scan_cluster_open(ctas);
+    if (rank == 0) scan_empty_sequences<V>(p, p.d_ht, p.dht_sn, p.d_h0, p.dh0_sn, c, mine);
+
+    float enter[V];  // u that enters the segment from the right
+#pragma unroll
+    for (int i = 0; i < V; ++i) enter[i] = 0.0f;
+
+    for (int k = 0; k < segments; ++k) {
+        const int turn = k & 1;
+        const int64_t t = first_token(k);
+        const uint32_t borders = scan_borders(p, t);
+        const bool plain = borders == 0 && t >= span.first && t + kScanSteps <= span.last;
+        float h[V];  // before this CTA's tokens
+        const int64_t tile = t / kScanChunk;
+        scan_load_state<V>(p.chunk, p.D, b * tiles + tile, c, mine && tile < tiles, h);
+        const bool there = flight.wait(warp, k);
+        const uint8_t *const px = piece(k), *const pg = px + RX::kBytes, *const pd = pg + RG::kBytes;
+        auto get_d = [&](int l) { return p.d_out ? RX::get(pd, l) : pack_zero<TX, V>(); };
+
+        float a[kScanSteps][V];
+        Pack<TX, V> x[kScanSteps], up[kScanSteps];
+        ScanMap<V> mh, mu;
+        mh.clear();
+        mu.clear();
+        if (plain) {
+#pragma unroll
+            for (int l = 0; l < kScanSteps; ++l) {
+                x[l] = RX::get(px, l);
+                up[l] = get_d(l);
+                vec_exp<TG, V>(RG::get(pg, l), a[l]);
+                float f[V];
+                vec_f32<TX, V>(x[l], f);
+                vec_mul<V>(mh.a, a[l], mh.a);
+                vec_fma<V>(a[l], mh.b, f, mh.b);
+            }
+#pragma unroll
+            for (int l = kScanSteps - 1; l >= 0; --l) {
+                float f[V];
+                vec_f32<TX, V>(up[l], f);
+                vec_add<V>(mu.b, f, f);
+                vec_mul<V>(a[l], f, mu.b);
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) mu.a[i] = mh.a[i];
+            fetch(k + kScanStages);
+        } else {
+#pragma unroll 1
+            for (int l = 0; l < kScanSteps; ++l) {
+                const int64_t at = t + l;
+                if (at < span.first || at >= span.last) {
+                    mh.cut_to_zero();
+                    continue;
+                }
+                if (borders >> l & 1) {
+                    scan_load_state<V>(p.h0, p.h0_sn, scan_sequence(p, b, at), c, mine, mh.b);
+                    mh.cut = true;
+                }
+                float f[V];
+                vec_f32<TX, V>(RX::get(px, l), f);
+                vec_exp<TG, V>(RG::get(pg, l), a[0]);
+                vec_mul<V>(mh.a, a[0], mh.a);
+                vec_fma<V>(a[0], mh.b, f, mh.b);
+            }
+#pragma unroll 1
+            for (int l = kScanSteps - 1; l >= 0; --l) {
+                const int64_t at = t + l;
+                if (at < span.first || at >= span.last) {
+                    mu.cut_to_zero();
+                    continue;
+                }
+                if (borders >> (l + 1) & 1) {
+                    scan_load_state<V>(p.d_ht, p.dht_sn, scan_sequence(p, b, at), c, mine, mu.b);
+                    mu.cut = true;
+                }
+                float f[V];
+                vec_f32<TX, V>(get_d(l), f);
+                vec_exp<TG, V>(RG::get(pg, l), a[0]);
+                vec_mul<V>(mu.a, a[0], mu.a);
+                vec_add<V>(mu.b, f, f);
+                vec_mul<V>(a[0], f, mu.b);
+            }
+        }
+        if (!there) mh.b[0] = mu.b[0] = __int_as_float(0x7fffffff);
+
+        *warps_h.at(turn, warp) = ScanSlot<V>(mh);
+        *warps_u.at(turn, warp) = ScanSlot<V>(mu);
+        __syncthreads();
+#pragma unroll 1
+        for (int w = 0; w < warp; ++w) ScanMap<V>(*warps_h.at(turn, w)).apply(h);
+        ScanMap<V> after, all;
+        scan_join_warps<V, true>(warps_u, turn, warp, after, all);
+        float u[V];
+        if (p.cluster == 1) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) u[i] = enter[i];
+            all.apply(enter);
+        } else {
+            scan_join_cluster<V, true>(ctas, k, p.cluster, rank, all, enter, u, &flight.lost);
+        }
+        after.apply(u);
+
+        float before[kScanSteps][V];  // h_{t-1}
+        if (plain) {
+#pragma unroll
+            for (int l = 0; l < kScanSteps; ++l) {
+                float f[V];
+                vec_f32<TX, V>(x[l], f);
+#pragma unroll
+                for (int i = 0; i < V; ++i) before[l][i] = h[i];
+                vec_fma<V>(a[l], h, f, h);
+            }
+#pragma unroll
+            for (int l = kScanSteps - 1; l >= 0; --l) {
+                float f[V], dgv[V];
+                vec_f32<TX, V>(up[l], f);
+                vec_add<V>(u, f, f);
+                vec_mul<V>(a[l], f, u);
+                vec_mul<V>(u, before[l], dgv);
+                if (mine && dx) scan_store<TX, V>(dx, p.dx_st, t, l, f);
+                if (mine && dg) scan_store<TG, V>(dg, p.dg_st, t, l, dgv);
+            }
+        } else {
+            float earlier[kScanSteps][V];  // as `before`, indexed by a loop that is not unrolled
+#pragma unroll 1
+            for (int l = 0; l < kScanSteps; ++l) {
+                const int64_t at = t + l;
+                if (at < span.first || at >= span.last) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) h[i] = 0.0f;
+                    continue;
+                }
+                if (borders >> l & 1) scan_load_state<V>(p.h0, p.h0_sn, scan_sequence(p, b, at), c, mine, h);
+                float f[V];
+                vec_f32<TX, V>(RX::get(px, l), f);
+                vec_exp<TG, V>(RG::get(pg, l), a[0]);
+#pragma unroll
+                for (int i = 0; i < V; ++i) earlier[l][i] = h[i];
+                vec_fma<V>(a[0], h, f, h);
+            }
+#pragma unroll 1
+            for (int l = kScanSteps - 1; l >= 0; --l) {
+                const int64_t at = t + l;
+                if (at >= p.T) continue;
+                float dh[V], dgv[V];
+                if (at < span.first || at >= span.last) {
+#pragma unroll
+                    for (int i = 0; i < V; ++i) u[i] = dh[i] = dgv[i] = 0.0f;
+                } else {
+                    if (borders >> (l + 1) & 1)
+                        scan_load_state<V>(p.d_ht, p.dht_sn, scan_sequence(p, b, at), c, mine, u);
+                    vec_f32<TX, V>(get_d(l), dh);
+                    vec_exp<TG, V>(RG::get(pg, l), a[0]);
+                    vec_add<V>(u, dh, dh);
+                    vec_mul<V>(a[0], dh, u);
+                    vec_mul<V>(u, earlier[l], dgv);
+                    if (p.d_h0 && (borders >> l & 1))
+                        scan_store_state<V>(p.d_h0, p.dh0_sn, scan_sequence(p, b, at), c, mine, u);
+                }
+                if (mine && dx) scan_store<TX, V>(dx, p.dx_st, t, l, dh);
+                if (mine && dg) scan_store<TG, V>(dg, p.dg_st, t, l, dgv);
+            }
+            fetch(k + kScanStages);
+        }
+    }
+    if (p.cluster > 1) scan_cluster_sync();
 }
 
 }  // namespace cgdr

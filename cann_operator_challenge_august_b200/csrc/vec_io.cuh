@@ -31,6 +31,15 @@ struct alignas(sizeof(T) * V) Pack {
     T e[V];
 };
 
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> pack_zero()
+{
+    Pack<T, V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.e[i] = from_f32<T>(0.0f);
+    return r;
+}
+
 template <typename T, int V, bool ALIGNED>
 __device__ __forceinline__ Pack<T, V> load_pack(const T* p, int valid = V)
 {
@@ -45,12 +54,32 @@ __device__ __forceinline__ Pack<T, V> load_pack(const T* p, int valid = V)
     return r;
 }
 
+// Two values at once: one conversion instruction for the 16-bit types.
+template <typename T> __device__ __forceinline__ void from_f32x2(float a, float b, T* to)
+{
+    to[0] = from_f32<T>(a);
+    to[1] = from_f32<T>(b);
+}
+template <> __device__ __forceinline__ void from_f32x2<__nv_bfloat16>(float a, float b, __nv_bfloat16* to)
+{
+    *reinterpret_cast<__nv_bfloat162*>(to) = __floats2bfloat162_rn(a, b);
+}
+template <> __device__ __forceinline__ void from_f32x2<__half>(float a, float b, __half* to)
+{
+    *reinterpret_cast<__half2*>(to) = __floats2half2_rn(a, b);
+}
+
 template <typename T, int V, bool ALIGNED>
 __device__ __forceinline__ void store_pack(T* p, const float* v, int valid = V)
 {
     Pack<T, V> r;
+    if constexpr (V % 2 == 0) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) r.e[i] = from_f32<T>(v[i]);
+        for (int i = 0; i < V; i += 2) from_f32x2<T>(v[i], v[i + 1], &r.e[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) r.e[i] = from_f32<T>(v[i]);
+    }
     if constexpr (ALIGNED) {
         using Raw = typename RawOf<sizeof(T) * V>::type;
         *reinterpret_cast<Raw*>(p) = *reinterpret_cast<const Raw*>(&r);
