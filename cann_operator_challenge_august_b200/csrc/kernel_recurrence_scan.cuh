@@ -58,6 +58,88 @@ struct ScanParams {
 // that row addresses are formed once a warp.
 __device__ __forceinline__ int scan_warp() { return __shfl_sync(~0u, static_cast<int>(threadIdx.x / 32), 0); }
 
+// ---- a lane's V channels: one fp32 register, or a pair for the packed instructions ------------
+
+template <int V> struct Vec;
+
+template <> struct Vec<1> {
+    float v;
+    static __device__ __forceinline__ Vec of(float x) { return {x}; }
+    __device__ __forceinline__ float get(int) const { return v; }
+    __device__ __forceinline__ void set(int, float x) { v = x; }
+};
+__device__ __forceinline__ Vec<1> vec_fma(Vec<1> a, Vec<1> b, Vec<1> c) { return {fmaf(a.v, b.v, c.v)}; }
+__device__ __forceinline__ Vec<1> operator*(Vec<1> a, Vec<1> b) { return {a.v * b.v}; }
+__device__ __forceinline__ Vec<1> operator+(Vec<1> a, Vec<1> b) { return {a.v + b.v}; }
+
+template <> struct Vec<2> {
+    uint64_t v;
+    static __device__ __forceinline__ Vec of(float x) { return pair(x, x); }
+    static __device__ __forceinline__ Vec pair(float a, float b)
+    {
+        Vec r;
+        asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+        return r;
+    }
+    __device__ __forceinline__ float get(int i) const
+    {
+        float a, b;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+        return i ? b : a;
+    }
+    __device__ __forceinline__ void set(int i, float x) { *this = i ? pair(get(0), x) : pair(x, get(1)); }
+};
+__device__ __forceinline__ Vec<2> vec_fma(Vec<2> a, Vec<2> b, Vec<2> c)
+{
+    Vec<2> r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ Vec<2> operator*(Vec<2> a, Vec<2> b)
+{
+    Vec<2> r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Vec<2> operator+(Vec<2> a, Vec<2> b)
+{
+    Vec<2> r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+
+template <typename T>
+__device__ __forceinline__ Vec<1> vec_of(const Pack<T, 1>& p)
+{
+    return {to_f32(p.e[0])};
+}
+__device__ __forceinline__ Vec<2> vec_of(const Pack<float, 2>& p) { return Vec<2>::pair(p.e[0], p.e[1]); }
+__device__ __forceinline__ Vec<2> vec_of(const Pack<__half, 2>& p)
+{
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p));
+    return Vec<2>::pair(f.x, f.y);
+}
+__device__ __forceinline__ Vec<2> vec_of(const Pack<__nv_bfloat16, 2>& p)
+{
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(&p);
+    return Vec<2>::pair(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+
+// exp(g): by the hardware's exponential (within 2 ulp; the argument's own
+// rounding adds |g| half-ulps); results below 2^-126 are 0.
+__device__ __forceinline__ float scan_exp2(float x)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ Vec<1> vec_exp(Vec<1> g) { return {scan_exp2(g.v * 1.4426950408889634f)}; }
+__device__ __forceinline__ Vec<2> vec_exp(Vec<2> g)
+{
+    const Vec<2> x = g * Vec<2>::of(1.4426950408889634f);
+    return Vec<2>::pair(scan_exp2(x.get(0)), scan_exp2(x.get(1)));
+}
+
 // ---- sequences ------------------------------------------------------------------------
 
 struct ScanSpan {
@@ -100,21 +182,23 @@ __device__ __forceinline__ int64_t scan_sequence(const ScanParams& p, int64_t b,
     return n < 0 ? 0 : n < p.N ? n : p.N - 1;
 }
 
+// Channels c .. c + V of row n of a [N, D] fp32 tensor (zeros without one).
 template <int V>
-__device__ __forceinline__ void scan_load_state(const float* base, int64_t stride, int64_t n, int64_t c, bool mine,
-                                                float* out)
+__device__ __forceinline__ Vec<V> scan_load_state(const float* base, int64_t stride, int64_t n, int64_t c, bool mine)
 {
+    Vec<V> r = Vec<V>::of(0.0f);
+    if (base && mine)
 #pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = base && mine ? base[n * stride + c + i] : 0.0f;
+        for (int i = 0; i < V; ++i) r.set(i, base[n * stride + c + i]);
+    return r;
 }
 
 template <int V>
-__device__ __forceinline__ void scan_store_state(float* base, int64_t stride, int64_t n, int64_t c, bool mine,
-                                                 const float* v)
+__device__ __forceinline__ void scan_store_state(float* base, int64_t stride, int64_t n, int64_t c, bool mine, Vec<V> v)
 {
     if (!base || !mine) return;
 #pragma unroll
-    for (int i = 0; i < V; ++i) base[n * stride + c + i] = v[i];
+    for (int i = 0; i < V; ++i) base[n * stride + c + i] = v.get(i);
 }
 
 // States of empty sequences pass through (`to` from `from`).
@@ -125,86 +209,19 @@ __device__ __forceinline__ void scan_empty_sequences(const ScanParams& p, const 
     if (!p.cu || !to) return;
     for (int64_t n = threadIdx.x / 32; n < p.N; n += kScanWarps) {
         if (p.cu[n + 1] > p.cu[n]) continue;
-        float h[V];
-        scan_load_state<V>(from, from_s, n, c, mine, h);
-        scan_store_state<V>(to, to_s, n, c, mine, h);
+        scan_store_state<V>(to, to_s, n, c, mine, scan_load_state<V>(from, from_s, n, c, mine));
     }
-}
-
-// ---- arithmetic on a lane's V channels, two at a time where V is even -----------------------
-
-__device__ __forceinline__ uint64_t f32x2(float a, float b)
-{
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void f32x2_split(uint64_t v, float& a, float& b)
-{
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-}
-
-template <int V>
-__device__ __forceinline__ void vec_fma(const float* a, const float* b, const float* c, float* to)
-{
-    if constexpr (V == 2) {
-        uint64_t r;
-        asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(f32x2(a[0], a[1])), "l"(f32x2(b[0], b[1])), "l"(f32x2(c[0], c[1])));
-        f32x2_split(r, to[0], to[1]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) to[i] = fmaf(a[i], b[i], c[i]);
-    }
-}
-template <int V>
-__device__ __forceinline__ void vec_mul(const float* a, const float* b, float* to)
-{
-    if constexpr (V == 2) {
-        uint64_t r;
-        asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f32x2(a[0], a[1])), "l"(f32x2(b[0], b[1])));
-        f32x2_split(r, to[0], to[1]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) to[i] = a[i] * b[i];
-    }
-}
-template <int V>
-__device__ __forceinline__ void vec_add(const float* a, const float* b, float* to)
-{
-    if constexpr (V == 2) {
-        uint64_t r;
-        asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(f32x2(a[0], a[1])), "l"(f32x2(b[0], b[1])));
-        f32x2_split(r, to[0], to[1]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) to[i] = a[i] + b[i];
-    }
-}
-template <typename T, int V>
-__device__ __forceinline__ void vec_f32(const Pack<T, V>& p, float* to)
-{
-#pragma unroll
-    for (int i = 0; i < V; ++i) to[i] = to_f32(p.e[i]);
-}
-// exp(g): by the hardware's exponential (within 2 ulp; the argument's own
-// rounding adds |g| half-ulps); results below 2^-126 are 0.
-template <typename T, int V>
-__device__ __forceinline__ void vec_exp(const Pack<T, V>& g, float* to)
-{
-    float x[V];
-    vec_f32<T, V>(g, x);
-    if constexpr (V == 2) {
-        const float log2e[2] = {1.4426950408889634f, 1.4426950408889634f};
-        vec_mul<V>(x, log2e, x);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) x[i] *= 1.4426950408889634f;
-    }
-#pragma unroll
-    for (int i = 0; i < V; ++i) asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(to[i]) : "f"(x[i]));
 }
 
 // ---- the ring: each warp's own 16 rows -------------------------------------------------------
+
+// Row `l` behind `row`, rows `step` bytes apart.
+__device__ __forceinline__ uint64_t scan_row(uint64_t row, uint32_t step, uint32_t l)
+{
+    uint64_t r;
+    asm("mad.wide.u32 %0, %1, %2, %3;" : "=l"(r) : "r"(step), "r"(l), "l"(row));
+    return r;
+}
 
 // Rows of 32 V channels of one tensor, and how a warp brings 16 of them in.
 template <typename T, int V, bool TMA>
@@ -228,7 +245,7 @@ struct ScanRows {
     static __device__ __forceinline__ void fetch(const T* base, int64_t stride, int64_t t, int64_t end, uint8_t* to)
     {
         const int lane = threadIdx.x % 32;
-        const uint8_t* const row = reinterpret_cast<const uint8_t*>(base + t * stride) + lane * kLane;
+        const uint64_t row = reinterpret_cast<uint64_t>(base + t * stride) + lane * kLane;
         const uint32_t step = static_cast<uint32_t>(stride) * sizeof(T);  // below 2^27: checked by the host
         const int count = end - t >= kScanSteps ? kScanSteps : end > t ? static_cast<int>(end - t) : 0;
         to += lane * kLane;
@@ -236,21 +253,21 @@ struct ScanRows {
             const uint32_t at = smem_u32(to);
             if (count == kScanSteps) {
 #pragma unroll
-                for (int l = 0; l < kScanSteps; ++l) copy(at + l * 32 * kLane, row + l * step);
+                for (int l = 0; l < kScanSteps; ++l) copy(at + l * 32 * kLane, scan_row(row, step, l));
             } else {
-                for (int l = 0; l < count; ++l) copy(at + l * 32 * kLane, row + l * step);
+                for (int l = 0; l < count; ++l) copy(at + l * 32 * kLane, scan_row(row, step, l));
             }
         } else {  // two bytes: too small for cp.async
             T e[kScanSteps];
 #pragma unroll
             for (int l = 0; l < kScanSteps; ++l)
-                if (l < count) e[l] = *reinterpret_cast<const T*>(row + l * step);
+                if (l < count) e[l] = *reinterpret_cast<const T*>(scan_row(row, step, l));
 #pragma unroll
             for (int l = 0; l < kScanSteps; ++l)
                 if (l < count) *reinterpret_cast<T*>(to + l * 32 * kLane) = e[l];
         }
     }
-    static __device__ __forceinline__ void copy(uint32_t to, const uint8_t* from)
+    static __device__ __forceinline__ void copy(uint32_t to, uint64_t from)
     {
         asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(kLane) : "memory");
     }
@@ -288,11 +305,14 @@ __device__ __forceinline__ bool scan_await(uint64_t* bar, uint32_t parity, volat
 
 // This lane's elements of row `l` behind `base` (token t of the slab).
 template <typename T, int V>
-__device__ __forceinline__ void scan_store(T* base, int64_t stride, int64_t t, int l, const float* v)
+__device__ __forceinline__ void scan_store(T* base, int64_t stride, int64_t t, int l, Vec<V> v)
 {
     const uint32_t step = static_cast<uint32_t>(stride) * sizeof(T);
-    uint8_t* const row = reinterpret_cast<uint8_t*>(base + t * stride) + threadIdx.x % 32 * (sizeof(T) * V);
-    store_pack<T, V, true>(reinterpret_cast<T*>(row + l * step), v);
+    const uint64_t row = reinterpret_cast<uint64_t>(base + t * stride) + threadIdx.x % 32 * (sizeof(T) * V);
+    float f[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = v.get(i);
+    store_pack<T, V, true>(reinterpret_cast<T*>(scan_row(row, step, l)), f);
 }
 
 // ---- joining ------------------------------------------------------------------------------
@@ -300,36 +320,31 @@ __device__ __forceinline__ void scan_store(T* base, int64_t stride, int64_t t, i
 // What a warp or a CTA does to the value that enters it: cut ? b : a v + b.
 template <int V>
 struct ScanMap {
-    float a[V], b[V];
+    Vec<V> a, b;
     bool cut;
     __device__ __forceinline__ void clear()
     {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            a[i] = 1.0f;
-            b[i] = 0.0f;
-        }
+        a = Vec<V>::of(1.0f);
+        b = Vec<V>::of(0.0f);
         cut = false;
     }
-    __device__ __forceinline__ void cut_to_zero()
+    // the value is `v` here, whatever entered
+    __device__ __forceinline__ void restart(Vec<V> v)
     {
-#pragma unroll
-        for (int i = 0; i < V; ++i) b[i] = 0.0f;
+        b = v;
         cut = true;
     }
-    __device__ __forceinline__ void apply(float* v) const
+    __device__ __forceinline__ Vec<V> operator()(Vec<V> v) const
     {
-        float r[V];
-        vec_fma<V>(a, v, b, r);
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = cut ? b[i] : r[i];
+        const Vec<V> r = vec_fma(a, v, b);
+        return cut ? b : r;
     }
     // this, then `next`
     __device__ __forceinline__ void then(const ScanMap& next)
     {
-        next.apply(b);
+        b = next(b);
         cut |= next.cut;
-        vec_mul<V>(a, next.a, a);
+        a = a * next.a;
     }
 };
 
@@ -342,18 +357,20 @@ struct alignas(8 * V) ScanSlot {
     {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            a[i] = m.a[i];
-            b[i] = m.b[i];
+            a[i] = m.a.get(i);
+            b[i] = m.b.get(i);
         }
         if (m.cut) a[0] = -1.0f;
     }
     __device__ __forceinline__ operator ScanMap<V>() const
     {
         ScanMap<V> m;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            m.a[i] = a[i];
-            m.b[i] = b[i];
+        if constexpr (V == 2) {
+            m.a = Vec<2>::pair(a[0], a[1]);
+            m.b = Vec<2>::pair(b[0], b[1]);
+        } else {
+            m.a = Vec<1>::of(a[0]);
+            m.b = Vec<1>::of(b[0]);
         }
         m.cut = a[0] < 0.0f;
         return m;
@@ -419,7 +436,7 @@ __device__ __forceinline__ void scan_send(ScanSlot<V>* to, uint64_t* bar, int ra
 // map of the segment between, which it sends when all its warps have read.
 template <int V, bool REVERSE>
 __device__ __forceinline__ void scan_join_cluster(ScanCluster<V>& s, int k, int ctas, int rank, const ScanMap<V>& mine,
-                                                  float* value, float* enters, volatile bool* lost)
+                                                  Vec<V>& value, Vec<V>& enters, volatile bool* lost)
 {
     const int turn = k & 1;
     if (threadIdx.x == 0) mbar_arrive_expect_tx(&s.full[turn], ctas * 32 * sizeof(ScanSlot<V>));
@@ -430,16 +447,10 @@ __device__ __forceinline__ void scan_join_cluster(ScanCluster<V>& s, int k, int 
 #pragma unroll 2
     for (int n = 0; n < ctas; ++n) {
         const int r = REVERSE ? ctas - 1 - n : n;
-        if (r == rank) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) enters[i] = value[i];
-        }
-        ScanMap<V>(*s.maps.at(turn, r)).apply(value);
+        if (r == rank) enters = value;
+        value = ScanMap<V>(*s.maps.at(turn, r))(value);
     }
-    if (!there) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) value[i] = enters[i] = __int_as_float(0x7fffffff);
-    }
+    if (!there) value = enters = Vec<V>::of(__int_as_float(0x7fffffff));
 }
 
 // From the warps' maps of a CTA in their order, or the reverse: what all do,
@@ -552,9 +563,7 @@ __global__ void __launch_bounds__(kScanThreads, 4)
     if (p.cluster > 1) scan_cluster_open(ctas);
     if (rank == 0) scan_empty_sequences<V>(p, p.h0, p.h0_sn, p.ht, p.ht_sn, c, mine);
 
-    float state[V];  // what enters the segment
-#pragma unroll
-    for (int i = 0; i < V; ++i) state[i] = 0.0f;
+    Vec<V> state = Vec<V>::of(0.0f);  // what enters the segment
 
     for (int seg = 0; seg < segments; ++seg) {
         const int turn = seg & 1;
@@ -565,16 +574,16 @@ __global__ void __launch_bounds__(kScanThreads, 4)
         const bool there = flight.wait(warp, seg);
         const uint8_t *const px = piece(seg), *const pg = px + RX::kBytes;
 
-        float a[kScanSteps][V], x[kScanSteps][V];
+        Vec<V> a[kScanSteps], x[kScanSteps];
         ScanMap<V> m;
         m.clear();
         if (plain) {
 #pragma unroll
             for (int l = 0; l < kScanSteps; ++l) {
-                vec_f32<TX, V>(RX::get(px, l), x[l]);
-                vec_exp<TG, V>(RG::get(pg, l), a[l]);
-                vec_mul<V>(m.a, a[l], m.a);
-                vec_fma<V>(a[l], m.b, x[l], m.b);
+                x[l] = vec_of(RX::get(px, l));
+                a[l] = vec_exp(vec_of(RG::get(pg, l)));
+                m.a = m.a * a[l];
+                m.b = vec_fma(a[l], m.b, x[l]);
             }
             fetch(seg + kScanStages);
         } else {
@@ -582,41 +591,37 @@ __global__ void __launch_bounds__(kScanThreads, 4)
             for (int l = 0; l < kScanSteps; ++l) {
                 const int64_t at = t + l;
                 if (at < span.first || at >= span.last) {  // no sequence's, or no token: the state is 0
-                    m.cut_to_zero();
+                    m.restart(Vec<V>::of(0.0f));
                     continue;
                 }
-                if (borders >> l & 1) {
-                    scan_load_state<V>(p.h0, p.h0_sn, scan_sequence(p, b, at), c, mine, m.b);
-                    m.cut = true;
-                }
-                vec_f32<TX, V>(RX::get(px, l), x[0]);
-                vec_exp<TG, V>(RG::get(pg, l), a[0]);
-                vec_mul<V>(m.a, a[0], m.a);
-                vec_fma<V>(a[0], m.b, x[0], m.b);
+                if (borders >> l & 1)
+                    m.restart(scan_load_state<V>(p.h0, p.h0_sn, scan_sequence(p, b, at), c, mine));
+                const Vec<V> f = vec_exp(vec_of(RG::get(pg, l)));
+                m.a = m.a * f;
+                m.b = vec_fma(f, m.b, vec_of(RX::get(px, l)));
             }
         }
-        if (!there) m.b[0] = __int_as_float(0x7fffffff);
+        if (!there) m.b = Vec<V>::of(__int_as_float(0x7fffffff));
 
         *warps.at(turn, warp) = ScanSlot<V>(m);
         __syncthreads();
         ScanMap<V> before, all;
         scan_join_warps<V, false>(warps, turn, warp, before, all);
-        float h[V];
+        Vec<V> h;
         if (p.cluster == 1) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) h[i] = state[i];
-            all.apply(state);
+            h = state;
+            state = all(state);
         } else {
             scan_join_cluster<V, false>(ctas, seg, p.cluster, rank, all, state, h, &flight.lost);
         }
-        before.apply(h);
+        h = before(h);
 
         if (p.chunk && warp == 0 && mine && t < p.T)
             scan_store_state<V>(p.chunk, p.D, b * tiles + t / kScanChunk, c, mine, h);
         if (plain) {
 #pragma unroll
             for (int l = 0; l < kScanSteps; ++l) {
-                vec_fma<V>(a[l], h, x[l], h);
+                h = vec_fma(a[l], h, x[l]);
                 if (mine) scan_store<TX, V>(out, p.o_st, t, l, h);
             }
         } else {
@@ -624,13 +629,10 @@ __global__ void __launch_bounds__(kScanThreads, 4)
             for (int l = 0; l < kScanSteps && t + l < p.T; ++l) {
                 const int64_t at = t + l;
                 if (at < span.first || at >= span.last) {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) h[i] = 0.0f;
+                    h = Vec<V>::of(0.0f);
                 } else {
-                    if (borders >> l & 1) scan_load_state<V>(p.h0, p.h0_sn, scan_sequence(p, b, at), c, mine, h);
-                    vec_f32<TX, V>(RX::get(px, l), x[0]);
-                    vec_exp<TG, V>(RG::get(pg, l), a[0]);
-                    vec_fma<V>(a[0], h, x[0], h);
+                    if (borders >> l & 1) h = scan_load_state<V>(p.h0, p.h0_sn, scan_sequence(p, b, at), c, mine);
+                    h = vec_fma(vec_exp(vec_of(RG::get(pg, l))), h, vec_of(RX::get(px, l)));
                     if (p.ht && (borders >> (l + 1) & 1))
                         scan_store_state<V>(p.ht, p.ht_sn, scan_sequence(p, b, at), c, mine, h);
                 }
@@ -711,158 +713,122 @@ __global__ void __launch_bounds__(kScanThreads, 3)
     if (p.cluster > 1) scan_cluster_open(ctas);
     if (rank == 0) scan_empty_sequences<V>(p, p.d_ht, p.dht_sn, p.d_h0, p.dh0_sn, c, mine);
 
-    float enter[V];  // u that enters the segment from the right
-#pragma unroll
-    for (int i = 0; i < V; ++i) enter[i] = 0.0f;
+    Vec<V> enter = Vec<V>::of(0.0f);  // u that enters the segment from the right
 
     for (int k = 0; k < segments; ++k) {
         const int turn = k & 1;
         const int64_t t = first_token(k);
         const uint32_t borders = scan_borders(p, t);
         const bool plain = borders == 0 && t >= span.first && t + kScanSteps <= span.last;
-        float h[V];  // before this CTA's tokens
         const int64_t tile = t / kScanChunk;
-        scan_load_state<V>(p.chunk, p.D, b * tiles + tile, c, mine && tile < tiles, h);
+        Vec<V> h = scan_load_state<V>(p.chunk, p.D, b * tiles + tile, c, mine && tile < tiles);  // before this CTA's tokens
         const bool there = flight.wait(warp, k);
         const uint8_t *const px = piece(k), *const pg = px + RX::kBytes, *const pd = pg + RG::kBytes;
-        auto get_d = [&](int l) { return p.d_out ? RX::get(pd, l) : pack_zero<TX, V>(); };
+        auto get_d = [&](int l) { return vec_of(p.d_out ? RX::get(pd, l) : pack_zero<TX, V>()); };
 
-        float a[kScanSteps][V];
-        Pack<TX, V> x[kScanSteps], up[kScanSteps];
+        Vec<V> a[kScanSteps], x[kScanSteps], up[kScanSteps];
         ScanMap<V> mh, mu;
         mh.clear();
         mu.clear();
         if (plain) {
 #pragma unroll
             for (int l = 0; l < kScanSteps; ++l) {
-                x[l] = RX::get(px, l);
+                x[l] = vec_of(RX::get(px, l));
                 up[l] = get_d(l);
-                vec_exp<TG, V>(RG::get(pg, l), a[l]);
-                float f[V];
-                vec_f32<TX, V>(x[l], f);
-                vec_mul<V>(mh.a, a[l], mh.a);
-                vec_fma<V>(a[l], mh.b, f, mh.b);
+                a[l] = vec_exp(vec_of(RG::get(pg, l)));
+                mh.a = mh.a * a[l];
+                mh.b = vec_fma(a[l], mh.b, x[l]);
             }
 #pragma unroll
-            for (int l = kScanSteps - 1; l >= 0; --l) {
-                float f[V];
-                vec_f32<TX, V>(up[l], f);
-                vec_add<V>(mu.b, f, f);
-                vec_mul<V>(a[l], f, mu.b);
-            }
-#pragma unroll
-            for (int i = 0; i < V; ++i) mu.a[i] = mh.a[i];
+            for (int l = kScanSteps - 1; l >= 0; --l) mu.b = a[l] * (mu.b + up[l]);
+            mu.a = mh.a;
             fetch(k + kScanStages);
         } else {
 #pragma unroll 1
             for (int l = 0; l < kScanSteps; ++l) {
                 const int64_t at = t + l;
                 if (at < span.first || at >= span.last) {
-                    mh.cut_to_zero();
+                    mh.restart(Vec<V>::of(0.0f));
                     continue;
                 }
-                if (borders >> l & 1) {
-                    scan_load_state<V>(p.h0, p.h0_sn, scan_sequence(p, b, at), c, mine, mh.b);
-                    mh.cut = true;
-                }
-                float f[V];
-                vec_f32<TX, V>(RX::get(px, l), f);
-                vec_exp<TG, V>(RG::get(pg, l), a[0]);
-                vec_mul<V>(mh.a, a[0], mh.a);
-                vec_fma<V>(a[0], mh.b, f, mh.b);
+                if (borders >> l & 1)
+                    mh.restart(scan_load_state<V>(p.h0, p.h0_sn, scan_sequence(p, b, at), c, mine));
+                const Vec<V> f = vec_exp(vec_of(RG::get(pg, l)));
+                mh.a = mh.a * f;
+                mh.b = vec_fma(f, mh.b, vec_of(RX::get(px, l)));
             }
 #pragma unroll 1
             for (int l = kScanSteps - 1; l >= 0; --l) {
                 const int64_t at = t + l;
                 if (at < span.first || at >= span.last) {
-                    mu.cut_to_zero();
+                    mu.restart(Vec<V>::of(0.0f));
                     continue;
                 }
-                if (borders >> (l + 1) & 1) {
-                    scan_load_state<V>(p.d_ht, p.dht_sn, scan_sequence(p, b, at), c, mine, mu.b);
-                    mu.cut = true;
-                }
-                float f[V];
-                vec_f32<TX, V>(get_d(l), f);
-                vec_exp<TG, V>(RG::get(pg, l), a[0]);
-                vec_mul<V>(mu.a, a[0], mu.a);
-                vec_add<V>(mu.b, f, f);
-                vec_mul<V>(a[0], f, mu.b);
+                if (borders >> (l + 1) & 1)
+                    mu.restart(scan_load_state<V>(p.d_ht, p.dht_sn, scan_sequence(p, b, at), c, mine));
+                const Vec<V> f = vec_exp(vec_of(RG::get(pg, l)));
+                mu.a = mu.a * f;
+                mu.b = f * (mu.b + get_d(l));
             }
         }
-        if (!there) mh.b[0] = mu.b[0] = __int_as_float(0x7fffffff);
+        if (!there) mh.b = mu.b = Vec<V>::of(__int_as_float(0x7fffffff));
 
         *warps_h.at(turn, warp) = ScanSlot<V>(mh);
         *warps_u.at(turn, warp) = ScanSlot<V>(mu);
         __syncthreads();
 #pragma unroll 1
-        for (int w = 0; w < warp; ++w) ScanMap<V>(*warps_h.at(turn, w)).apply(h);
+        for (int w = 0; w < warp; ++w) h = ScanMap<V>(*warps_h.at(turn, w))(h);
         ScanMap<V> after, all;
         scan_join_warps<V, true>(warps_u, turn, warp, after, all);
-        float u[V];
+        Vec<V> u;
         if (p.cluster == 1) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) u[i] = enter[i];
-            all.apply(enter);
+            u = enter;
+            enter = all(enter);
         } else {
             scan_join_cluster<V, true>(ctas, k, p.cluster, rank, all, enter, u, &flight.lost);
         }
-        after.apply(u);
+        u = after(u);
 
-        float before[kScanSteps][V];  // h_{t-1}
         if (plain) {
 #pragma unroll
-            for (int l = 0; l < kScanSteps; ++l) {
-                float f[V];
-                vec_f32<TX, V>(x[l], f);
-#pragma unroll
-                for (int i = 0; i < V; ++i) before[l][i] = h[i];
-                vec_fma<V>(a[l], h, f, h);
+            for (int l = 0; l < kScanSteps; ++l) {  // x_t gives way to h_{t-1}
+                const Vec<V> next = vec_fma(a[l], h, x[l]);
+                x[l] = h;
+                h = next;
             }
 #pragma unroll
             for (int l = kScanSteps - 1; l >= 0; --l) {
-                float f[V], dgv[V];
-                vec_f32<TX, V>(up[l], f);
-                vec_add<V>(u, f, f);
-                vec_mul<V>(a[l], f, u);
-                vec_mul<V>(u, before[l], dgv);
-                if (mine && dx) scan_store<TX, V>(dx, p.dx_st, t, l, f);
-                if (mine && dg) scan_store<TG, V>(dg, p.dg_st, t, l, dgv);
+                const Vec<V> dh = u + up[l];
+                u = a[l] * dh;
+                if (mine && dx) scan_store<TX, V>(dx, p.dx_st, t, l, dh);
+                if (mine && dg) scan_store<TG, V>(dg, p.dg_st, t, l, u * x[l]);
             }
         } else {
-            float earlier[kScanSteps][V];  // as `before`, indexed by a loop that is not unrolled
+            Vec<V> earlier[kScanSteps];  // h_{t-1}
 #pragma unroll 1
             for (int l = 0; l < kScanSteps; ++l) {
                 const int64_t at = t + l;
                 if (at < span.first || at >= span.last) {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) h[i] = 0.0f;
+                    h = Vec<V>::of(0.0f);
                     continue;
                 }
-                if (borders >> l & 1) scan_load_state<V>(p.h0, p.h0_sn, scan_sequence(p, b, at), c, mine, h);
-                float f[V];
-                vec_f32<TX, V>(RX::get(px, l), f);
-                vec_exp<TG, V>(RG::get(pg, l), a[0]);
-#pragma unroll
-                for (int i = 0; i < V; ++i) earlier[l][i] = h[i];
-                vec_fma<V>(a[0], h, f, h);
+                if (borders >> l & 1) h = scan_load_state<V>(p.h0, p.h0_sn, scan_sequence(p, b, at), c, mine);
+                earlier[l] = h;
+                h = vec_fma(vec_exp(vec_of(RG::get(pg, l))), h, vec_of(RX::get(px, l)));
             }
 #pragma unroll 1
             for (int l = kScanSteps - 1; l >= 0; --l) {
                 const int64_t at = t + l;
                 if (at >= p.T) continue;
-                float dh[V], dgv[V];
+                Vec<V> dh = Vec<V>::of(0.0f), dgv = dh;
                 if (at < span.first || at >= span.last) {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) u[i] = dh[i] = dgv[i] = 0.0f;
+                    u = dh;
                 } else {
                     if (borders >> (l + 1) & 1)
-                        scan_load_state<V>(p.d_ht, p.dht_sn, scan_sequence(p, b, at), c, mine, u);
-                    vec_f32<TX, V>(get_d(l), dh);
-                    vec_exp<TG, V>(RG::get(pg, l), a[0]);
-                    vec_add<V>(u, dh, dh);
-                    vec_mul<V>(a[0], dh, u);
-                    vec_mul<V>(u, earlier[l], dgv);
+                        u = scan_load_state<V>(p.d_ht, p.dht_sn, scan_sequence(p, b, at), c, mine);
+                    dh = u + get_d(l);
+                    u = vec_exp(vec_of(RG::get(pg, l))) * dh;
+                    dgv = u * earlier[l];
                     if (p.d_h0 && (borders >> l & 1))
                         scan_store_state<V>(p.d_h0, p.dh0_sn, scan_sequence(p, b, at), c, mine, u);
                 }
