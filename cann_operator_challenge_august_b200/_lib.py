@@ -35,7 +35,7 @@ DEVICE_WAIT_TIMEOUT = 0x1
 DEVICE_BAD_VARLEN = 0x2
 DEVICE_BAD_STATE_INDEX = 0x4
 
-RECURRENCE_CHUNK = 64  # CGDR_RECURRENCE_CHUNK
+RECURRENCE_CHUNK = 128  # CGDR_RECURRENCE_CHUNK
 
 # Every symbol declared in include/*.h, by header.
 EXPORTS_BY_HEADER = {

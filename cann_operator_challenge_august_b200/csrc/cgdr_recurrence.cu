@@ -226,19 +226,21 @@ cgdrStatus check_chunks(const cgdrTensor* t, ScanParams* p)
     if ((st = check_rank(t, 3, "chunk_states"))) return st;
     if (t->dtype != CGDR_DT_FLOAT32) return fail(CGDR_STATUS_BAD_DTYPE, "chunk_states must be float32");
     if (!shape_is(t, {p->B, (p->T + kScanChunk - 1) / kScanChunk, p->D}))
-        return fail(CGDR_STATUS_BAD_SHAPE, "chunk_states must have shape [B, ceil(T/64), D]");
+        return fail(CGDR_STATUS_BAD_SHAPE, "chunk_states must have shape [B, ceil(T/128), D]");
     if ((st = check_contiguous(t, "chunk_states"))) return st;
     p->chunk = static_cast<float*>(t->data);
     return CGDR_STATUS_SUCCESS;
 }
 
+// Warps of a CTA; a CTA's tile of a segment is 16 tokens a warp.
+constexpr int kScanW = 8;
+
 // CTAs of a cluster, which share a slab's tokens: doubled while all CTAs still
-// fit on the GPU at once (`resident` CTAs an SM) and have a chunk each.
-int32_t scan_cluster(const ScanParams& p, int64_t slabs, int64_t resident)
+// fit on the GPU at once (`resident` CTAs an SM) and have a tile each.
+int32_t scan_cluster(const ScanParams& p, int64_t slabs, int most, int64_t resident)
 {
-    const int64_t tiles = (p.T + kScanChunk - 1) / kScanChunk;
     int32_t c = 1;
-    while (c < kScanMaxCluster && 2 * c <= tiles && 2 * c * slabs <= 148 * resident) c *= 2;
+    while (c < most && c * kScanW * kScanSteps < p.T && 2 * c * slabs <= 148 * resident) c *= 2;
     return c;
 }
 
@@ -264,16 +266,18 @@ cgdrStatus scan_map(const cgdrTensor* t, int V, CUtensorMap* map, const char* na
 }
 
 template <typename K>
-cudaError_t launch_scan(K kernel, ScanParams& p, const ScanMapsTma& maps, int V, int smem, int64_t resident,
+cudaError_t launch_scan(K kernel, ScanParams& p, const ScanMapsTma& maps, int V, int smem, int cluster,
                         cudaStream_t stream)
 {
-    // the maps of 4 warps (twice, backwards) and 8 CTAs; 1 KB is the system's
-    const int64_t fit = 227 * 1024 / (smem + V * 8192 + 1024 + 128);
+    // two CTAs an SM by registers, one where shared memory does not hold two:
+    // the ring, the maps of warps and CTAs, and 1 KB of the system's
+    int64_t resident = 2;
+    const int64_t fit = 227 * 1024 / (smem + V * 512 * (kScanW + kScanW / 2 + cluster) + 256 + 1024);
     if (resident > fit) resident = fit;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     const int64_t slabs = (p.D + 32 * V - 1) / (32 * V);
-    p.cluster = scan_cluster(p, slabs * p.B, resident);
+    p.cluster = scan_cluster(p, slabs * p.B, cluster, resident);
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = static_cast<unsigned>(p.cluster);
@@ -281,7 +285,7 @@ cudaError_t launch_scan(K kernel, ScanParams& p, const ScanMapsTma& maps, int V,
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(static_cast<unsigned>(slabs * p.cluster), static_cast<unsigned>(p.B));
-    cfg.blockDim = dim3(kScanThreads);
+    cfg.blockDim = dim3(32 * kScanW);
     cfg.dynamicSmemBytes = static_cast<size_t>(smem);
     cfg.stream = stream;
     cfg.attrs = &attr;
@@ -289,8 +293,10 @@ cudaError_t launch_scan(K kernel, ScanParams& p, const ScanMapsTma& maps, int V,
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<const ScanParams>(p), maps);
 }
 
-// How the rows are read: two channels a lane by TMA; two by cp.async where
-// rows are no multiple of 16 bytes (of a lane's 4 or 8, then); one otherwise.
+// How the rows are read: by TMA with two channels a lane, by cp.async with two
+// where rows are no multiple of 16 bytes, else one channel a lane.  (Four
+// channels a lane, 256-byte rows of 16-bit types, leave one CTA an SM and were
+// slower: 382 against 302 us forwards on 65536 x 4096.)
 enum class ScanPath { kTma, kPairs, kSingle };
 
 struct ScanLaunch {
@@ -303,10 +309,10 @@ struct ScanLaunch {
     template <typename TX, typename TG, int V, bool TMA>
     void go()
     {
-        error = backward ? launch_scan(scan_backward_kernel<TX, TG, V, TMA>, p, maps, V, scan_backward_smem<TX, TG, V>(),
-                                       3, stream)
-                         : launch_scan(scan_forward_kernel<TX, TG, V, TMA>, p, maps, V, scan_forward_smem<TX, TG, V>(),
-                                       4, stream);
+        error = backward ? launch_scan(scan_backward_kernel<TX, TG, V, kScanW, TMA>, p, maps, V,
+                                       scan_backward_smem<TX, TG, V, kScanW>(), kScanBackwardCluster, stream)
+                         : launch_scan(scan_forward_kernel<TX, TG, V, kScanW, TMA>, p, maps, V,
+                                       scan_forward_smem<TX, TG, V, kScanW>(), kScanForwardCluster, stream);
     }
     template <typename TX, typename TG>
     void operator()()

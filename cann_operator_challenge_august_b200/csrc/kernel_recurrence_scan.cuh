@@ -2,8 +2,8 @@
 // (include/cgdr_recurrence.h).
 //
 // One cluster of CTAs walks along the tokens of one slab of 32 V channels, a
-// segment of 64 tokens a CTA at a time; a lane owns V channels, a warp 16
-// consecutive tokens of its CTA's 64.  Per segment:
+// segment at a time; a lane owns V channels, a warp 16 consecutive tokens of
+// the segment, a CTA of W warps 16 W.  Per segment:
 //   1. every warp runs its 16 steps from a zero state and keeps the factor
 //      A = prod exp(g) and the end state B, so that the true end state is
 //      A h_in + B;
@@ -19,7 +19,7 @@
 //
 // Backwards, the same with u_t = exp(g_{t+1}) dh_{t+1} folded from the right
 // (the factors A are the same), and with h_{t-1} recomputed from the state
-// that the forward pass saved before each 64 tokens.
+// that the forward pass saved before each 128 tokens.
 //
 // Sequences.  At a sequence's first token the running state is replaced by
 // its initial state, at its last token (backwards) u by d_final_state; a warp
@@ -36,11 +36,11 @@
 
 namespace cgdr {
 
-constexpr int kScanChunk = 64;    // CGDR_RECURRENCE_CHUNK: tokens of a CTA and segment
-constexpr int kScanWarps = 4;
-constexpr int kScanThreads = kScanWarps * 32;
-constexpr int kScanSteps = kScanChunk / kScanWarps;
-constexpr int kScanMaxCluster = 8;
+constexpr int kScanSteps = 16;     // tokens of a warp and segment; a CTA of W warps has 16 W
+constexpr int kScanChunk = 128;    // CGDR_RECURRENCE_CHUNK: tokens between saved states
+// CTAs of a cluster at most; backwards fewer, so that two CTAs' shared memory
+// fits an SM
+constexpr int kScanForwardCluster = 8, kScanBackwardCluster = 4;
 
 struct ScanParams {
     const void *x, *g, *d_out;
@@ -58,119 +58,112 @@ struct ScanParams {
 // that row addresses are formed once a warp.
 __device__ __forceinline__ int scan_warp() { return __shfl_sync(~0u, static_cast<int>(threadIdx.x / 32), 0); }
 
-// ---- a lane's V channels: one fp32 register, or a pair for the packed instructions ------------
+// ---- a lane's V channels -------------------------------------------------------------------
+// (The packed fp32x2 instructions were tried here: fewer instructions, the same
+// time, as each takes the place of two.)
 
-template <int V> struct Vec;
-
-template <> struct Vec<1> {
-    float v;
-    static __device__ __forceinline__ Vec of(float x) { return {x}; }
-    __device__ __forceinline__ float get(int) const { return v; }
-    __device__ __forceinline__ void set(int, float x) { v = x; }
-};
-__device__ __forceinline__ Vec<1> vec_fma(Vec<1> a, Vec<1> b, Vec<1> c) { return {fmaf(a.v, b.v, c.v)}; }
-__device__ __forceinline__ Vec<1> operator*(Vec<1> a, Vec<1> b) { return {a.v * b.v}; }
-__device__ __forceinline__ Vec<1> operator+(Vec<1> a, Vec<1> b) { return {a.v + b.v}; }
-
-template <> struct Vec<2> {
-    uint64_t v;
-    static __device__ __forceinline__ Vec of(float x) { return pair(x, x); }
-    static __device__ __forceinline__ Vec pair(float a, float b)
+template <int V>
+struct Vec {
+    float v[V];
+    static __device__ __forceinline__ Vec of(float x)
     {
         Vec r;
-        asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+#pragma unroll
+        for (int i = 0; i < V; ++i) r.v[i] = x;
         return r;
     }
-    __device__ __forceinline__ float get(int i) const
-    {
-        float a, b;
-        asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
-        return i ? b : a;
-    }
-    __device__ __forceinline__ void set(int i, float x) { *this = i ? pair(get(0), x) : pair(x, get(1)); }
 };
-__device__ __forceinline__ Vec<2> vec_fma(Vec<2> a, Vec<2> b, Vec<2> c)
+template <int V>
+__device__ __forceinline__ Vec<V> vec_fma(Vec<V> a, Vec<V> b, Vec<V> c)
 {
-    Vec<2> r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    Vec<V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = fmaf(a.v[i], b.v[i], c.v[i]);
     return r;
 }
-__device__ __forceinline__ Vec<2> operator*(Vec<2> a, Vec<2> b)
+template <int V>
+__device__ __forceinline__ Vec<V> operator*(Vec<V> a, Vec<V> b)
 {
-    Vec<2> r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    Vec<V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = a.v[i] * b.v[i];
     return r;
 }
-__device__ __forceinline__ Vec<2> operator+(Vec<2> a, Vec<2> b)
+template <int V>
+__device__ __forceinline__ Vec<V> operator+(Vec<V> a, Vec<V> b)
 {
-    Vec<2> r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    Vec<V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = a.v[i] + b.v[i];
     return r;
 }
 
-template <typename T>
-__device__ __forceinline__ Vec<1> vec_of(const Pack<T, 1>& p)
+template <typename T, int V>
+__device__ __forceinline__ Vec<V> vec_of(const Pack<T, V>& p)
 {
-    return {to_f32(p.e[0])};
-}
-__device__ __forceinline__ Vec<2> vec_of(const Pack<float, 2>& p) { return Vec<2>::pair(p.e[0], p.e[1]); }
-__device__ __forceinline__ Vec<2> vec_of(const Pack<__half, 2>& p)
-{
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p));
-    return Vec<2>::pair(f.x, f.y);
-}
-__device__ __forceinline__ Vec<2> vec_of(const Pack<__nv_bfloat16, 2>& p)
-{
-    const uint32_t u = *reinterpret_cast<const uint32_t*>(&p);
-    return Vec<2>::pair(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+    Vec<V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = to_f32(p.e[i]);
+    return r;
 }
 
 // exp(g): by the hardware's exponential (within 2 ulp; the argument's own
 // rounding adds |g| half-ulps); results below 2^-126 are 0.
-__device__ __forceinline__ float scan_exp2(float x)
+template <int V>
+__device__ __forceinline__ Vec<V> vec_exp(Vec<V> g)
 {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    Vec<V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r.v[i]) : "f"(g.v[i] * 1.4426950408889634f));
     return r;
-}
-__device__ __forceinline__ Vec<1> vec_exp(Vec<1> g) { return {scan_exp2(g.v * 1.4426950408889634f)}; }
-__device__ __forceinline__ Vec<2> vec_exp(Vec<2> g)
-{
-    const Vec<2> x = g * Vec<2>::of(1.4426950408889634f);
-    return Vec<2>::pair(scan_exp2(x.get(0)), scan_exp2(x.get(1)));
 }
 
 // ---- sequences ------------------------------------------------------------------------
 
-struct ScanSpan {
+// What a warp knows of the sequences' borders (cu_seqlens, or 0 and T), as it
+// walks along the tokens 16 at a time.  The nearest border ahead is kept, so
+// cu_seqlens is searched only where one lies in the 16 tokens.
+struct ScanBorders {
     int64_t first, last;  // tokens [first, last) belong to sequences
+    int64_t ahead;
+    __device__ __forceinline__ ScanBorders(const ScanParams& p, bool reverse)
+        : first(0), last(p.T), ahead(reverse ? INT64_MAX : INT64_MIN)
+    {
+        if (p.cu) {
+            first = p.cu[0];
+            const int64_t end = p.cu[p.N];
+            last = end < p.T ? end : p.T;
+        }
+    }
+    // Bit i: a sequence begins or ends before token t + i, 0 <= i <= 16.
+    template <bool REVERSE>
+    __device__ __forceinline__ uint32_t at(const ScanParams& p, int64_t t)
+    {
+        if (REVERSE ? ahead < t : ahead > t + kScanSteps) return 0;
+        uint32_t bits = 0;
+        unsigned near = 0xffffffffu;  // distance of the nearest border past the 17 places
+        const int64_t n = p.cu ? p.N : 1;
+        for (int64_t i = threadIdx.x % 32; i <= n; i += 32) {
+            const int64_t d = (p.cu ? p.cu[i] : i ? p.T : 0) - t;
+            if (d >= 0 && d <= kScanSteps) bits |= 1u << d;
+            const int64_t far = REVERSE ? -d : d - kScanSteps;
+            if (far > 0 && far < near) near = static_cast<unsigned>(far);
+        }
+        near = __reduce_min_sync(~0u, near);
+        ahead = REVERSE ? t - near : t + kScanSteps + near;
+        return __reduce_or_sync(~0u, bits);
+    }
+    // Bit i: token t + i belongs to no sequence.
+    __device__ __forceinline__ uint32_t dead(int64_t t) const
+    {
+        constexpr uint32_t all = (1u << kScanSteps) - 1;
+        const int64_t from = first - t, to = last - t;
+        const uint32_t before = from <= 0 ? 0 : from >= kScanSteps ? all : (1u << from) - 1;
+        const uint32_t upto = to <= 0 ? 0 : to >= kScanSteps ? all : (1u << to) - 1;
+        return (before | ~upto) & all;
+    }
 };
-
-__device__ __forceinline__ ScanSpan scan_span(const ScanParams& p)
-{
-    ScanSpan s{0, p.T};
-    if (p.cu) {
-        s.first = p.cu[0];
-        const int64_t last = p.cu[p.N];
-        s.last = last < p.T ? last : p.T;
-    }
-    return s;
-}
-
-// Bit i: a sequence begins or ends before token t + i, 0 <= i <= 16.
-__device__ __forceinline__ uint32_t scan_borders(const ScanParams& p, int64_t t)
-{
-    if (!p.cu) {
-        const int64_t to_end = p.T - t;
-        return (t == 0 ? 1u : 0u) | (to_end >= 0 && to_end <= kScanSteps ? 1u << to_end : 0u);
-    }
-    uint32_t bits = 0;
-    for (int64_t i = threadIdx.x % 32; i <= p.N; i += 32) {
-        const int64_t d = p.cu[i] - t;
-        if (d >= 0 && d <= kScanSteps) bits |= 1u << d;
-    }
-    return __reduce_or_sync(~0u, bits);
-}
 
 // The sequence of token t: the last one that begins at or before it.
 __device__ __forceinline__ int64_t scan_sequence(const ScanParams& p, int64_t b, int64_t t)
@@ -189,7 +182,7 @@ __device__ __forceinline__ Vec<V> scan_load_state(const float* base, int64_t str
     Vec<V> r = Vec<V>::of(0.0f);
     if (base && mine)
 #pragma unroll
-        for (int i = 0; i < V; ++i) r.set(i, base[n * stride + c + i]);
+        for (int i = 0; i < V; ++i) r.v[i] = base[n * stride + c + i];
     return r;
 }
 
@@ -198,16 +191,31 @@ __device__ __forceinline__ void scan_store_state(float* base, int64_t stride, in
 {
     if (!base || !mine) return;
 #pragma unroll
-    for (int i = 0; i < V; ++i) base[n * stride + c + i] = v.get(i);
+    for (int i = 0; i < V; ++i) base[n * stride + c + i] = v.v[i];
+}
+
+// The same for the sequence of token t; kept out of line, since few warps meet
+// a border.
+template <int V>
+__device__ __noinline__ Vec<V> scan_load_of(const ScanParams& p, const float* base, int64_t stride, int64_t b, int64_t t,
+                                            int64_t c, bool mine)
+{
+    return scan_load_state<V>(base, stride, scan_sequence(p, b, t), c, mine);
+}
+template <int V>
+__device__ __noinline__ void scan_store_of(const ScanParams& p, float* base, int64_t stride, int64_t b, int64_t t,
+                                           int64_t c, bool mine, Vec<V> v)
+{
+    scan_store_state<V>(base, stride, scan_sequence(p, b, t), c, mine, v);
 }
 
 // States of empty sequences pass through (`to` from `from`).
-template <int V>
+template <int V, int W>
 __device__ __forceinline__ void scan_empty_sequences(const ScanParams& p, const float* from, int64_t from_s, float* to,
                                                      int64_t to_s, int64_t c, bool mine)
 {
     if (!p.cu || !to) return;
-    for (int64_t n = threadIdx.x / 32; n < p.N; n += kScanWarps) {
+    for (int64_t n = threadIdx.x / 32; n < p.N; n += W) {
         if (p.cu[n + 1] > p.cu[n]) continue;
         scan_store_state<V>(to, to_s, n, c, mine, scan_load_state<V>(from, from_s, n, c, mine));
     }
@@ -303,17 +311,23 @@ __device__ __forceinline__ bool scan_await(uint64_t* bar, uint32_t parity, volat
     return false;
 }
 
-// This lane's elements of row `l` behind `base` (token t of the slab).
+// This lane's elements of an output's rows of 32 V channels from one token on.
 template <typename T, int V>
-__device__ __forceinline__ void scan_store(T* base, int64_t stride, int64_t t, int l, Vec<V> v)
-{
-    const uint32_t step = static_cast<uint32_t>(stride) * sizeof(T);
-    const uint64_t row = reinterpret_cast<uint64_t>(base + t * stride) + threadIdx.x % 32 * (sizeof(T) * V);
-    float f[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = v.get(i);
-    store_pack<T, V, true>(reinterpret_cast<T*>(scan_row(row, step, l)), f);
-}
+struct ScanOut {
+    uint64_t row;
+    uint32_t step;
+    bool mine;
+    __device__ __forceinline__ ScanOut(T* slab, int64_t stride, int64_t t, bool lane_in)
+        : row(reinterpret_cast<uint64_t>(slab + t * stride) + threadIdx.x % 32 * (sizeof(T) * V)),
+          step(static_cast<uint32_t>(stride) * sizeof(T)),
+          mine(lane_in && slab)
+    {
+    }
+    __device__ __forceinline__ void put(int l, Vec<V> v) const
+    {
+        if (mine) store_pack<T, V, true>(reinterpret_cast<T*>(scan_row(row, step, l)), v.v);
+    }
+};
 
 // ---- joining ------------------------------------------------------------------------------
 
@@ -336,8 +350,7 @@ struct ScanMap {
     }
     __device__ __forceinline__ Vec<V> operator()(Vec<V> v) const
     {
-        const Vec<V> r = vec_fma(a, v, b);
-        return cut ? b : r;
+        return cut ? b : vec_fma(a, v, b);
     }
     // this, then `next`
     __device__ __forceinline__ void then(const ScanMap& next)
@@ -349,7 +362,7 @@ struct ScanMap {
 };
 
 // A lane's part of a map on its way through shared memory: one access of 8 V
-// bytes.  A factor is never negative, so a[0] = -1 tells that the map cuts.
+// bytes.  A factor is never negative, so the sign of a[0] tells that the map cuts.
 template <int V>
 struct alignas(8 * V) ScanSlot {
     float a[V], b[V];
@@ -357,23 +370,45 @@ struct alignas(8 * V) ScanSlot {
     {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            a[i] = m.a.get(i);
-            b[i] = m.b.get(i);
+            a[i] = m.a.v[i];
+            b[i] = m.b.v[i];
         }
-        if (m.cut) a[0] = -1.0f;
+        if (m.cut) a[0] = -a[0];
     }
     __device__ __forceinline__ operator ScanMap<V>() const
     {
         ScanMap<V> m;
-        if constexpr (V == 2) {
-            m.a = Vec<2>::pair(a[0], a[1]);
-            m.b = Vec<2>::pair(b[0], b[1]);
-        } else {
-            m.a = Vec<1>::of(a[0]);
-            m.b = Vec<1>::of(b[0]);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            m.a.v[i] = i == 0 ? fabsf(a[i]) : a[i];
+            m.b.v[i] = b[i];
         }
-        m.cut = a[0] < 0.0f;
+        m.cut = __float_as_int(a[0]) < 0;
         return m;
+    }
+};
+
+// The h map of a warp going backwards, beside its u map, which has the same
+// factors: only what it adds, and whether it cuts (uniform in the warp).
+template <int V, int K>
+struct ScanAdds {
+    alignas(16) float b[2][K][32 * V];
+    int cut[2][K];
+    __device__ __forceinline__ void put(int turn, int k, const ScanMap<V>& m)
+    {
+        const int lane = threadIdx.x % 32;
+#pragma unroll
+        for (int i = 0; i < V; ++i) b[turn][k][lane * V + i] = m.b.v[i];
+        if (lane == 0) cut[turn][k] = m.cut;
+    }
+    __device__ __forceinline__ Vec<V> apply(int turn, int k, const ScanMap<V>& u, Vec<V> v) const
+    {
+        const int lane = threadIdx.x % 32;
+        ScanMap<V> m;
+        m.a = u.a;
+        m.b = vec_of(load_pack<float, V, true>(&b[turn][k][lane * V]));
+        m.cut = cut[turn][k];
+        return m(v);
     }
 };
 
@@ -390,9 +425,9 @@ struct ScanMaps {
 
 // The same for the CTAs of a cluster, with a barrier for each turn that counts
 // the bytes which the CTAs (this one too) send.
-template <int V>
+template <int V, int K>
 struct ScanCluster {
-    ScanMaps<V, kScanMaxCluster> maps;
+    ScanMaps<V, K> maps;
     alignas(8) uint64_t full[2];
 };
 
@@ -401,8 +436,8 @@ __device__ __forceinline__ void scan_cluster_sync()
     asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
-template <int V>
-__device__ __forceinline__ void scan_cluster_open(ScanCluster<V>& s)
+template <int V, int K>
+__device__ __forceinline__ void scan_cluster_open(ScanCluster<V, K>& s)
 {
     if (threadIdx.x == 0) {
         mbar_init(&s.full[0], 1);
@@ -419,14 +454,16 @@ __device__ __forceinline__ void scan_send(ScanSlot<V>* to, uint64_t* bar, int ra
     uint32_t at, b;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(to)), "r"(rank));
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(smem_u32(bar)), "r"(rank));
-    if constexpr (V == 2)
+    if constexpr (V > 1) {
+        static_assert(V == 2, "one vector of four");
         asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(at),
                      "f"(v.a[0]), "f"(v.a[1]), "f"(v.b[0]), "f"(v.b[1]), "r"(b)
                      : "memory");
-    else
+    } else {
         asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(at),
                      "f"(v.a[0]), "f"(v.b[0]), "r"(b)
                      : "memory");
+    }
 }
 
 // Folds `value` (what enters segment k) through the CTAs of the cluster in
@@ -434,14 +471,14 @@ __device__ __forceinline__ void scan_send(ScanSlot<V>* to, uint64_t* bar, int ra
 // `value` is what leaves the segment.  `mine` is the whole CTA's map.  A map's
 // slots are written again two segments later, by CTAs that have this CTA's
 // map of the segment between, which it sends when all its warps have read.
-template <int V, bool REVERSE>
-__device__ __forceinline__ void scan_join_cluster(ScanCluster<V>& s, int k, int ctas, int rank, const ScanMap<V>& mine,
+template <int V, int W, bool REVERSE, int K>
+__device__ __forceinline__ void scan_join_cluster(ScanCluster<V, K>& s, int k, int ctas, int rank, const ScanMap<V>& mine,
                                                   Vec<V>& value, Vec<V>& enters, volatile bool* lost)
 {
     const int turn = k & 1;
     if (threadIdx.x == 0) mbar_arrive_expect_tx(&s.full[turn], ctas * 32 * sizeof(ScanSlot<V>));
     const ScanSlot<V> slot(mine);
-    for (int to = scan_warp(); to < ctas; to += kScanWarps)
+    for (int to = scan_warp(); to < ctas; to += W)
         scan_send<V>(s.maps.at(turn, rank), &s.full[turn], to, slot);
     const bool there = scan_await(&s.full[turn], k >> 1 & 1, lost);
 #pragma unroll 2
@@ -454,30 +491,70 @@ __device__ __forceinline__ void scan_join_cluster(ScanCluster<V>& s, int k, int 
 }
 
 // From the warps' maps of a CTA in their order, or the reverse: what all do,
-// and what those before this warp do.
-template <int V, bool REVERSE>
-__device__ __forceinline__ void scan_join_warps(ScanMaps<V, kScanWarps>& maps, int turn, int warp, ScanMap<V>& before,
+// and what those before this warp do.  `cuts`: one of them may cut.
+template <int V, int W, bool REVERSE>
+__device__ __forceinline__ void scan_join_warps(ScanMaps<V, W>& maps, int turn, int warp, bool cuts, ScanMap<V>& before,
                                                 ScanMap<V>& all)
 {
-    ScanMap<V> m[kScanWarps];
-#pragma unroll
-    for (int w = 0; w < kScanWarps; ++w) m[w] = *maps.at(turn, REVERSE ? kScanWarps - 1 - w : w);
     all.clear();
-#pragma unroll
-    for (int w = 0; w < kScanWarps; ++w) {
-        if (w == (REVERSE ? kScanWarps - 1 - warp : warp)) before = all;
-        all.then(m[w]);
+    before.clear();
+    if (cuts) {
+#pragma unroll 1
+        for (int n = 0; n < W; ++n) {
+            const int w = REVERSE ? W - 1 - n : n;
+            if (w == warp) before = all;
+            all.then(*maps.at(turn, w));
+        }
+        return;
     }
+    ScanMap<V> m[W];
+#pragma unroll
+    for (int n = 0; n < W; ++n) m[n] = *maps.at(turn, REVERSE ? W - 1 - n : n);
+#pragma unroll
+    for (int n = 0; n < W; ++n) {
+        if (n == (REVERSE ? W - 1 - warp : warp)) {
+            before.a = all.a;
+            before.b = all.b;
+        }
+        all.b = vec_fma(m[n].a, all.b, m[n].b);
+        all.a = all.a * m[n].a;
+    }
+}
+
+// The same where the CTA is alone: what enters this warp, and `value` from
+// what enters the segment to what leaves it.
+template <int V, int W, bool REVERSE>
+__device__ __forceinline__ Vec<V> scan_fold_warps(ScanMaps<V, W>& maps, int turn, int warp, bool cuts, Vec<V>& value)
+{
+    Vec<V> enters = value;
+    if (cuts) {
+#pragma unroll 1
+        for (int n = 0; n < W; ++n) {
+            const int w = REVERSE ? W - 1 - n : n;
+            if (w == warp) enters = value;
+            value = ScanMap<V>(*maps.at(turn, w))(value);
+        }
+        return enters;
+    }
+    ScanMap<V> m[W];
+#pragma unroll
+    for (int n = 0; n < W; ++n) m[n] = *maps.at(turn, REVERSE ? W - 1 - n : n);
+#pragma unroll
+    for (int n = 0; n < W; ++n) {
+        if (n == (REVERSE ? W - 1 - warp : warp)) enters = value;
+        value = vec_fma(m[n].a, value, m[n].b);
+    }
+    return enters;
 }
 
 // ---- forwards -------------------------------------------------------------------------------
 
 constexpr int kScanStages = 2;
 
-// A CTA's copies: kScanStages x kScanWarps pieces of NT tensors' rows.
-template <int NT, bool TMA>
+// A CTA's copies: kScanStages pieces of rows for each of its W warps.
+template <int W, bool TMA>
 struct ScanFlight {
-    alignas(8) uint64_t full[TMA ? kScanStages : 1][kScanWarps];
+    alignas(8) uint64_t full[TMA ? kScanStages : 1][W];
     bool lost;  // a wait ran out
     __device__ __forceinline__ void open()
     {
@@ -485,7 +562,7 @@ struct ScanFlight {
             lost = false;
             if constexpr (TMA) {
 #pragma unroll
-                for (int i = 0; i < kScanStages * kScanWarps; ++i) mbar_init(&full[0][0] + i, 1);
+                for (int i = 0; i < kScanStages * W; ++i) mbar_init(&full[0][0] + i, 1);
                 fence_mbarrier_init();
             }
         }
@@ -504,37 +581,38 @@ struct ScanMapsTma {
     CUtensorMap x, g, d_out;  // [B, T, D] in boxes of 16 rows and 32 V channels
 };
 
-template <typename TX, typename TG, int V>
+template <typename TX, typename TG, int V, int W>
 constexpr int scan_forward_smem()
 {
-    return kScanStages * kScanWarps * (ScanRows<TX, V, true>::kBytes + ScanRows<TG, V, true>::kBytes);
+    return kScanStages * W * (ScanRows<TX, V, true>::kBytes + ScanRows<TG, V, true>::kBytes);
 }
 
-template <typename TX, typename TG, int V, bool TMA>
-__global__ void __launch_bounds__(kScanThreads, 4)
+template <typename TX, typename TG, int V, int W, bool TMA>
+__global__ void __launch_bounds__(W * 32, 16 / W)
     scan_forward_kernel(const ScanParams p, const __grid_constant__ ScanMapsTma maps)
 {
     using RX = ScanRows<TX, V, TMA>;
     using RG = ScanRows<TG, V, TMA>;
     constexpr int kPiece = RX::kBytes + RG::kBytes;
     extern __shared__ __align__(128) uint8_t ring[];
-    __shared__ ScanMaps<V, kScanWarps> warps;
-    __shared__ ScanCluster<V> ctas;
-    __shared__ ScanFlight<2, TMA> flight;
+    __shared__ ScanMaps<V, W> warps;
+    __shared__ ScanCluster<V, kScanForwardCluster> ctas;
+    __shared__ ScanFlight<W, TMA> flight;
 
     const int warp = scan_warp(), lane = threadIdx.x % 32;
     const int rank = blockIdx.x % p.cluster;
     const int64_t slab = static_cast<int64_t>(blockIdx.x / p.cluster) * 32 * V, c = slab + lane * V, b = blockIdx.y;
     const bool mine = c < p.D;
-    const int64_t tiles = (p.T + kScanChunk - 1) / kScanChunk;
-    const int segments = static_cast<int>((tiles + p.cluster - 1) / p.cluster);
-    const ScanSpan span = scan_span(p);
+    constexpr int kTile = W * kScanSteps;  // tokens of this CTA in a segment
+    const int segments = static_cast<int>((p.T + kTile * p.cluster - 1) / (kTile * p.cluster));
+    const int64_t chunks = (p.T + kScanChunk - 1) / kScanChunk;
+    ScanBorders seqs(p, false);
     TX* const out = static_cast<TX*>(p.out) + b * p.o_sb + slab;
 
     auto first_token = [&](int seg) {
-        return (static_cast<int64_t>(seg) * p.cluster + rank) * kScanChunk + warp * kScanSteps;
+        return (static_cast<int64_t>(seg) * p.cluster + rank) * kTile + warp * kScanSteps;
     };
-    auto piece = [&](int seg) { return ring + (seg % kScanStages * kScanWarps + warp) * kPiece; };
+    auto piece = [&](int seg) { return ring + (seg % kScanStages * W + warp) * kPiece; };
     auto fetch = [&](int seg) {
         uint8_t* const to = piece(seg);
         if constexpr (TMA) {
@@ -561,16 +639,15 @@ __global__ void __launch_bounds__(kScanThreads, 4)
 #pragma unroll
     for (int s = 0; s < kScanStages; ++s) fetch(s);
     if (p.cluster > 1) scan_cluster_open(ctas);
-    if (rank == 0) scan_empty_sequences<V>(p, p.h0, p.h0_sn, p.ht, p.ht_sn, c, mine);
+    if (rank == 0) scan_empty_sequences<V, W>(p, p.h0, p.h0_sn, p.ht, p.ht_sn, c, mine);
 
     Vec<V> state = Vec<V>::of(0.0f);  // what enters the segment
 
     for (int seg = 0; seg < segments; ++seg) {
         const int turn = seg & 1;
         const int64_t t = first_token(seg);
-        const uint32_t borders = scan_borders(p, t);
-        // nothing begins or ends in these steps, and all of them are a sequence's
-        const bool plain = borders == 0 && t >= span.first && t + kScanSteps <= span.last;
+        const uint32_t borders = seqs.at<false>(p, t), dead = seqs.dead(t);
+        const bool plain = (borders | dead) == 0;
         const bool there = flight.wait(warp, seg);
         const uint8_t *const px = piece(seg), *const pg = px + RX::kBytes;
 
@@ -585,60 +662,57 @@ __global__ void __launch_bounds__(kScanThreads, 4)
                 m.a = m.a * a[l];
                 m.b = vec_fma(a[l], m.b, x[l]);
             }
-            fetch(seg + kScanStages);
         } else {
-#pragma unroll 1
+#pragma unroll
             for (int l = 0; l < kScanSteps; ++l) {
-                const int64_t at = t + l;
-                if (at < span.first || at >= span.last) {  // no sequence's, or no token: the state is 0
-                    m.restart(Vec<V>::of(0.0f));
-                    continue;
+                x[l] = vec_of(RX::get(px, l));
+                a[l] = vec_exp(vec_of(RG::get(pg, l)));
+                if (dead >> l & 1) {  // no sequence's, or no token: the state is 0
+                    a[l] = Vec<V>::of(1.0f);
+                    x[l] = Vec<V>::of(0.0f);
+                    m.restart(x[l]);
+                } else if (borders >> l & 1) {
+                    m.restart(scan_load_of<V>(p, p.h0, p.h0_sn, b, t + l, c, mine));
                 }
-                if (borders >> l & 1)
-                    m.restart(scan_load_state<V>(p.h0, p.h0_sn, scan_sequence(p, b, at), c, mine));
-                const Vec<V> f = vec_exp(vec_of(RG::get(pg, l)));
-                m.a = m.a * f;
-                m.b = vec_fma(f, m.b, vec_of(RX::get(px, l)));
+                m.a = m.a * a[l];
+                m.b = vec_fma(a[l], m.b, x[l]);
             }
         }
+        fetch(seg + kScanStages);
         if (!there) m.b = Vec<V>::of(__int_as_float(0x7fffffff));
 
         *warps.at(turn, warp) = ScanSlot<V>(m);
-        __syncthreads();
-        ScanMap<V> before, all;
-        scan_join_warps<V, false>(warps, turn, warp, before, all);
+        const bool cuts = __syncthreads_or(m.cut);
         Vec<V> h;
         if (p.cluster == 1) {
-            h = state;
-            state = all(state);
+            h = scan_fold_warps<V, W, false>(warps, turn, warp, cuts, state);
         } else {
-            scan_join_cluster<V, false>(ctas, seg, p.cluster, rank, all, state, h, &flight.lost);
+            ScanMap<V> before, all;
+            scan_join_warps<V, W, false>(warps, turn, warp, cuts, before, all);
+            scan_join_cluster<V, W, false>(ctas, seg, p.cluster, rank, all, state, h, &flight.lost);
+            h = before(h);
         }
-        h = before(h);
 
-        if (p.chunk && warp == 0 && mine && t < p.T)
-            scan_store_state<V>(p.chunk, p.D, b * tiles + t / kScanChunk, c, mine, h);
+        if (p.chunk && warp == 0 && t % kScanChunk == 0 && t < p.T)
+            scan_store_state<V>(p.chunk, p.D, b * chunks + t / kScanChunk, c, mine, h);
+        const ScanOut<TX, V> to(out, p.o_st, t, mine);
         if (plain) {
 #pragma unroll
             for (int l = 0; l < kScanSteps; ++l) {
                 h = vec_fma(a[l], h, x[l]);
-                if (mine) scan_store<TX, V>(out, p.o_st, t, l, h);
+                to.put(l, h);
             }
         } else {
-#pragma unroll 1
-            for (int l = 0; l < kScanSteps && t + l < p.T; ++l) {
-                const int64_t at = t + l;
-                if (at < span.first || at >= span.last) {
-                    h = Vec<V>::of(0.0f);
-                } else {
-                    if (borders >> l & 1) h = scan_load_state<V>(p.h0, p.h0_sn, scan_sequence(p, b, at), c, mine);
-                    h = vec_fma(vec_exp(vec_of(RG::get(pg, l))), h, vec_of(RX::get(px, l)));
-                    if (p.ht && (borders >> (l + 1) & 1))
-                        scan_store_state<V>(p.ht, p.ht_sn, scan_sequence(p, b, at), c, mine, h);
-                }
-                if (mine) scan_store<TX, V>(out, p.o_st, t, l, h);
+#pragma unroll
+            for (int l = 0; l < kScanSteps; ++l) {
+                const bool out_of = dead >> l & 1;
+                if (out_of) h = Vec<V>::of(0.0f);
+                else if (borders >> l & 1) h = scan_load_of<V>(p, p.h0, p.h0_sn, b, t + l, c, mine);
+                h = vec_fma(a[l], h, x[l]);
+                if (t + l < p.T) to.put(l, h);
+                if (!out_of && p.ht && (borders >> (l + 1) & 1))
+                    scan_store_of<V>(p, p.ht, p.ht_sn, b, t + l, c, mine, h);
             }
-            fetch(seg + kScanStages);
         }
     }
     if (p.cluster > 1) scan_cluster_sync();  // none leaves while another may still send to it
@@ -646,39 +720,41 @@ __global__ void __launch_bounds__(kScanThreads, 4)
 
 // ---- backwards --------------------------------------------------------------------------------
 
-template <typename TX, typename TG, int V>
+template <typename TX, typename TG, int V, int W>
 constexpr int scan_backward_smem()
 {
-    return kScanStages * kScanWarps * (2 * ScanRows<TX, V, true>::kBytes + ScanRows<TG, V, true>::kBytes);
+    return kScanStages * W * (2 * ScanRows<TX, V, true>::kBytes + ScanRows<TG, V, true>::kBytes);
 }
 
-template <typename TX, typename TG, int V, bool TMA>
-__global__ void __launch_bounds__(kScanThreads, 3)
+template <typename TX, typename TG, int V, int W, bool TMA>
+__global__ void __launch_bounds__(W * 32, 16 / W)
     scan_backward_kernel(const ScanParams p, const __grid_constant__ ScanMapsTma maps)
 {
     using RX = ScanRows<TX, V, TMA>;
     using RG = ScanRows<TG, V, TMA>;
     constexpr int kPiece = 2 * RX::kBytes + RG::kBytes;
     extern __shared__ __align__(128) uint8_t ring[];
-    __shared__ ScanMaps<V, kScanWarps> warps_h, warps_u;
-    __shared__ ScanCluster<V> ctas;
-    __shared__ ScanFlight<3, TMA> flight;
+    __shared__ ScanMaps<V, W> warps_u;
+    __shared__ ScanAdds<V, W> warps_h;
+    __shared__ ScanCluster<V, kScanBackwardCluster> ctas;
+    __shared__ ScanFlight<W, TMA> flight;
 
     const int warp = scan_warp(), lane = threadIdx.x % 32;
     const int rank = blockIdx.x % p.cluster;
     const int64_t slab = static_cast<int64_t>(blockIdx.x / p.cluster) * 32 * V, c = slab + lane * V, b = blockIdx.y;
     const bool mine = c < p.D;
-    const int64_t tiles = (p.T + kScanChunk - 1) / kScanChunk;
-    const int segments = static_cast<int>((tiles + p.cluster - 1) / p.cluster);
-    const ScanSpan span = scan_span(p);
+    constexpr int kTile = W * kScanSteps;  // tokens of this CTA in a segment
+    const int segments = static_cast<int>((p.T + kTile * p.cluster - 1) / (kTile * p.cluster));
+    const int64_t chunks = (p.T + kScanChunk - 1) / kScanChunk;
+    ScanBorders seqs(p, true);
     TX* const dx = p.dx ? static_cast<TX*>(p.dx) + b * p.dx_sb + slab : nullptr;
     TG* const dg = p.dg ? static_cast<TG*>(p.dg) + b * p.dg_sb + slab : nullptr;
 
     // segments run from the last to the first: turn k is segment segments - 1 - k
     auto first_token = [&](int k) {
-        return (static_cast<int64_t>(segments - 1 - k) * p.cluster + rank) * kScanChunk + warp * kScanSteps;
+        return (static_cast<int64_t>(segments - 1 - k) * p.cluster + rank) * kTile + warp * kScanSteps;
     };
-    auto piece = [&](int k) { return ring + (k % kScanStages * kScanWarps + warp) * kPiece; };
+    auto piece = [&](int k) { return ring + (k % kScanStages * W + warp) * kPiece; };
     auto fetch = [&](int k) {
         uint8_t* const to = piece(k);
         if constexpr (TMA) {
@@ -711,132 +787,122 @@ __global__ void __launch_bounds__(kScanThreads, 3)
 #pragma unroll
     for (int s = 0; s < kScanStages; ++s) fetch(s);
     if (p.cluster > 1) scan_cluster_open(ctas);
-    if (rank == 0) scan_empty_sequences<V>(p, p.d_ht, p.dht_sn, p.d_h0, p.dh0_sn, c, mine);
+    if (rank == 0) scan_empty_sequences<V, W>(p, p.d_ht, p.dht_sn, p.d_h0, p.dh0_sn, c, mine);
 
     Vec<V> enter = Vec<V>::of(0.0f);  // u that enters the segment from the right
 
     for (int k = 0; k < segments; ++k) {
         const int turn = k & 1;
         const int64_t t = first_token(k);
-        const uint32_t borders = scan_borders(p, t);
-        const bool plain = borders == 0 && t >= span.first && t + kScanSteps <= span.last;
-        const int64_t tile = t / kScanChunk;
-        Vec<V> h = scan_load_state<V>(p.chunk, p.D, b * tiles + tile, c, mine && tile < tiles);  // before this CTA's tokens
+        const uint32_t borders = seqs.at<true>(p, t), dead = seqs.dead(t);
+        const bool plain = (borders | dead) == 0;
+        const int64_t chunk = t / kScanChunk;
+        Vec<V> h = scan_load_state<V>(p.chunk, p.D, b * chunks + chunk, c, mine && chunk < chunks);  // before this CTA's tokens
         const bool there = flight.wait(warp, k);
         const uint8_t *const px = piece(k), *const pg = px + RX::kBytes, *const pd = pg + RG::kBytes;
+        auto get_x = [&](int l) { return vec_of(RX::get(px, l)); };
+        auto get_a = [&](int l) { return vec_exp(vec_of(RG::get(pg, l))); };
         auto get_d = [&](int l) { return vec_of(p.d_out ? RX::get(pd, l) : pack_zero<TX, V>()); };
 
-        Vec<V> a[kScanSteps], x[kScanSteps], up[kScanSteps];
+        // u leaves as A u + sum over l of (a_0 .. a_l) d_l, so both maps come of
+        // one walk; x and d_out are read again from shared memory afterwards
+        // rather than kept, which leaves registers for twice the warps
+        Vec<V> a[kScanSteps];
         ScanMap<V> mh, mu;
         mh.clear();
         mu.clear();
         if (plain) {
 #pragma unroll
             for (int l = 0; l < kScanSteps; ++l) {
-                x[l] = vec_of(RX::get(px, l));
-                up[l] = get_d(l);
-                a[l] = vec_exp(vec_of(RG::get(pg, l)));
+                a[l] = get_a(l);
                 mh.a = mh.a * a[l];
-                mh.b = vec_fma(a[l], mh.b, x[l]);
+                mh.b = vec_fma(a[l], mh.b, get_x(l));
+                if (p.d_out) mu.b = vec_fma(mh.a, get_d(l), mu.b);
             }
-#pragma unroll
-            for (int l = kScanSteps - 1; l >= 0; --l) mu.b = a[l] * (mu.b + up[l]);
-            mu.a = mh.a;
-            fetch(k + kScanStages);
         } else {
-#pragma unroll 1
+#pragma unroll
             for (int l = 0; l < kScanSteps; ++l) {
-                const int64_t at = t + l;
-                if (at < span.first || at >= span.last) {
+                a[l] = get_a(l);
+                if (dead >> l & 1) {
+                    a[l] = Vec<V>::of(1.0f);
                     mh.restart(Vec<V>::of(0.0f));
+                    mu.cut = true;
                     continue;
                 }
-                if (borders >> l & 1)
-                    mh.restart(scan_load_state<V>(p.h0, p.h0_sn, scan_sequence(p, b, at), c, mine));
-                const Vec<V> f = vec_exp(vec_of(RG::get(pg, l)));
-                mh.a = mh.a * f;
-                mh.b = vec_fma(f, mh.b, vec_of(RX::get(px, l)));
-            }
-#pragma unroll 1
-            for (int l = kScanSteps - 1; l >= 0; --l) {
-                const int64_t at = t + l;
-                if (at < span.first || at >= span.last) {
-                    mu.restart(Vec<V>::of(0.0f));
-                    continue;
+                if (borders >> l & 1) mh.restart(scan_load_of<V>(p, p.h0, p.h0_sn, b, t + l, c, mine));
+                mh.a = mh.a * a[l];
+                mh.b = vec_fma(a[l], mh.b, get_x(l));
+                if (!mu.cut) {  // what lies right of the first sequence's end does not reach out
+                    mu.b = vec_fma(mh.a, get_d(l), mu.b);
+                    if (borders >> (l + 1) & 1) {
+                        mu.b = vec_fma(mh.a, scan_load_of<V>(p, p.d_ht, p.dht_sn, b, t + l, c, mine), mu.b);
+                        mu.cut = true;
+                    }
                 }
-                if (borders >> (l + 1) & 1)
-                    mu.restart(scan_load_state<V>(p.d_ht, p.dht_sn, scan_sequence(p, b, at), c, mine));
-                const Vec<V> f = vec_exp(vec_of(RG::get(pg, l)));
-                mu.a = mu.a * f;
-                mu.b = f * (mu.b + get_d(l));
             }
         }
+        mu.a = mh.a;
         if (!there) mh.b = mu.b = Vec<V>::of(__int_as_float(0x7fffffff));
 
-        *warps_h.at(turn, warp) = ScanSlot<V>(mh);
+        warps_h.put(turn, warp, mh);
         *warps_u.at(turn, warp) = ScanSlot<V>(mu);
-        __syncthreads();
+        const bool cuts = __syncthreads_or(mh.cut || mu.cut);
 #pragma unroll 1
-        for (int w = 0; w < warp; ++w) h = ScanMap<V>(*warps_h.at(turn, w))(h);
-        ScanMap<V> after, all;
-        scan_join_warps<V, true>(warps_u, turn, warp, after, all);
+        for (int w = 0; w < warp; ++w) h = warps_h.apply(turn, w, *warps_u.at(turn, w), h);
         Vec<V> u;
         if (p.cluster == 1) {
-            u = enter;
-            enter = all(enter);
+            u = scan_fold_warps<V, W, true>(warps_u, turn, warp, cuts, enter);
         } else {
-            scan_join_cluster<V, true>(ctas, k, p.cluster, rank, all, enter, u, &flight.lost);
+            ScanMap<V> after, all;
+            scan_join_warps<V, W, true>(warps_u, turn, warp, cuts, after, all);
+            scan_join_cluster<V, W, true>(ctas, k, p.cluster, rank, all, enter, u, &flight.lost);
+            u = after(u);
         }
-        u = after(u);
 
+        const ScanOut<TX, V> to_x(dx, p.dx_st, t, mine);
+        const ScanOut<TG, V> to_g(dg, p.dg_st, t, mine);
+        Vec<V> before[kScanSteps];  // h_{t-1}
         if (plain) {
 #pragma unroll
-            for (int l = 0; l < kScanSteps; ++l) {  // x_t gives way to h_{t-1}
-                const Vec<V> next = vec_fma(a[l], h, x[l]);
-                x[l] = h;
-                h = next;
+            for (int l = 0; l < kScanSteps; ++l) {
+                before[l] = h;
+                h = vec_fma(a[l], h, get_x(l));
             }
 #pragma unroll
             for (int l = kScanSteps - 1; l >= 0; --l) {
-                const Vec<V> dh = u + up[l];
+                const Vec<V> dh = p.d_out ? u + get_d(l) : u;
                 u = a[l] * dh;
-                if (mine && dx) scan_store<TX, V>(dx, p.dx_st, t, l, dh);
-                if (mine && dg) scan_store<TG, V>(dg, p.dg_st, t, l, u * x[l]);
+                to_x.put(l, dh);
+                to_g.put(l, u * before[l]);
             }
         } else {
-            Vec<V> earlier[kScanSteps];  // h_{t-1}
-#pragma unroll 1
+#pragma unroll
             for (int l = 0; l < kScanSteps; ++l) {
-                const int64_t at = t + l;
-                if (at < span.first || at >= span.last) {
-                    h = Vec<V>::of(0.0f);
-                    continue;
-                }
-                if (borders >> l & 1) h = scan_load_state<V>(p.h0, p.h0_sn, scan_sequence(p, b, at), c, mine);
-                earlier[l] = h;
-                h = vec_fma(vec_exp(vec_of(RG::get(pg, l))), h, vec_of(RX::get(px, l)));
+                before[l] = h;
+                if (dead >> l & 1) continue;
+                if (borders >> l & 1) before[l] = scan_load_of<V>(p, p.h0, p.h0_sn, b, t + l, c, mine);
+                h = vec_fma(a[l], before[l], get_x(l));
             }
-#pragma unroll 1
+#pragma unroll
             for (int l = kScanSteps - 1; l >= 0; --l) {
-                const int64_t at = t + l;
-                if (at >= p.T) continue;
                 Vec<V> dh = Vec<V>::of(0.0f), dgv = dh;
-                if (at < span.first || at >= span.last) {
+                if (dead >> l & 1) {
                     u = dh;
                 } else {
-                    if (borders >> (l + 1) & 1)
-                        u = scan_load_state<V>(p.d_ht, p.dht_sn, scan_sequence(p, b, at), c, mine);
+                    if (borders >> (l + 1) & 1) u = scan_load_of<V>(p, p.d_ht, p.dht_sn, b, t + l, c, mine);
                     dh = u + get_d(l);
-                    u = vec_exp(vec_of(RG::get(pg, l))) * dh;
-                    dgv = u * earlier[l];
+                    u = a[l] * dh;
+                    dgv = u * before[l];
                     if (p.d_h0 && (borders >> l & 1))
-                        scan_store_state<V>(p.d_h0, p.dh0_sn, scan_sequence(p, b, at), c, mine, u);
+                        scan_store_of<V>(p, p.d_h0, p.dh0_sn, b, t + l, c, mine, u);
                 }
-                if (mine && dx) scan_store<TX, V>(dx, p.dx_st, t, l, dh);
-                if (mine && dg) scan_store<TG, V>(dg, p.dg_st, t, l, dgv);
+                if (t + l < p.T) {
+                    to_x.put(l, dh);
+                    to_g.put(l, dgv);
+                }
             }
-            fetch(k + kScanStages);
         }
+        fetch(k + kScanStages);
     }
     if (p.cluster > 1) scan_cluster_sync();
 }

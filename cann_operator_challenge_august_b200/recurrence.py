@@ -213,7 +213,7 @@ def gated_linear_recurrence(
 
     Differentiable in x, g and initial_state (once).  The gradients are those
     of the recurrence in fp32, recomputed from x, g and one saved state per
-    64 tokens.  To capture a backward pass into a CUDA graph, capture its
+    128 tokens.  To capture a backward pass into a CUDA graph, capture its
     forward pass in the same graph."""
     if torch.is_grad_enabled() and (x.requires_grad or g.requires_grad
                                     or (initial_state is not None and initial_state.requires_grad)):

@@ -62,7 +62,7 @@ cgdrStatus cgdrRecurrentGatedDeltaRule(
 
 /* Tokens between two of the states that the forward pass saves for the
  * backward pass (chunk_states). */
-#define CGDR_RECURRENCE_CHUNK 64
+#define CGDR_RECURRENCE_CHUNK 128
 
 /* h_t = exp(g_t) h_{t-1} + x_t, channel by channel, out_t = h_t.
  *     x, out         [B, T, D]  bf16, fp16 or fp32
@@ -72,8 +72,8 @@ cgdrStatus cgdrRecurrentGatedDeltaRule(
  *     cu_seqlens     [N+1]      int64 from 0, non-decreasing, contiguous
  *                               (NULL: every batch row is one sequence, N = B);
  *                               needs B == 1
- *     chunk_states   [B, ceil(T/64), D]  fp32, contiguous: the state before
- *                               each 64-token chunk (NULL unless a backward
+ *     chunk_states   [B, ceil(T/128), D]  fp32, contiguous: the state
+ *                               before each 128-token chunk (NULL unless a backward
  *                               pass follows)
  * Rows of `out` behind the last sequence are zero.  The state is held in
  * fp32; out is rounded once.  An empty sequence's final state is its initial

@@ -261,7 +261,7 @@ def test_scan_writes_stay_inside(T, cu, D):
     lib, N = _lib.load(), 1 if cu is None else len(cu) - 1
     x, g = rand(1, T, D, seed=1, dtype=BF), gates(1, T, D, seed=2)
     cut = None if cu is None else torch.tensor(cu, device=dev())
-    outs = [guarded((1, T, D), BF), guarded((N, D), F32), guarded((1, -(-T // 64), D), F32)]
+    outs = [guarded((1, T, D), BF), guarded((N, D), F32), guarded((1, -(-T // 128), D), F32)]
     grads = [guarded((1, T, D), BF), guarded((1, T, D), F32), guarded((N, D), F32)]
     assert lib.cgdrGatedLinearRecurrence(_view(x), _view(g), None, _view(cut), *[_view(t) for t, _ in outs], None) == 0
     assert lib.cgdrGatedLinearRecurrenceBackward(_view(x), _view(g), None, _view(cut), _view(outs[2][0]), _view(x), None,
@@ -277,7 +277,7 @@ def test_scan_survives_inconsistent_bounds(cu):
     lib, T, D = _lib.load(), 100, 36
     x, g = rand(1, T, D, seed=1, dtype=BF), gates(1, T, D, seed=2)
     cut = torch.tensor(cu, device=dev())
-    outs = [guarded((1, T, D), BF), guarded((2, D), F32), guarded((1, 2, D), F32)]
+    outs = [guarded((1, T, D), BF), guarded((2, D), F32), guarded((1, 1, D), F32)]
     outs[2][0].zero_()
     grads = [guarded((1, T, D), BF), guarded((1, T, D), F32), guarded((2, D), F32)]
     assert lib.cgdrGatedLinearRecurrence(_view(x), _view(g), None, _view(cut), *[_view(t) for t, _ in outs], None) == 0

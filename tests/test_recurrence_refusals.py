@@ -84,7 +84,7 @@ def test_delta_refuses(over, status):
 
 def scan(**over):
     a = dict(x=E(2, 130, 24, dtype=BF), g=E(2, 130, 24), h0=E(2, 24), cu=None, out=E(2, 130, 24, dtype=BF), ht=E(2, 24),
-             chunks=E(2, 3, 24))
+             chunks=E(2, 2, 24))
     a.update(over)
     return _lib.load().cgdrGatedLinearRecurrence(
         *[_view(a[n]) for n in ("x", "g", "h0", "cu", "out", "ht", "chunks")], None)
@@ -92,7 +92,7 @@ def scan(**over):
 
 def packed(**over):
     a = dict(x=E(1, 130, 24, dtype=BF), g=E(1, 130, 24), h0=E(3, 24), cu=E(4, dtype=I64),
-             out=E(1, 130, 24, dtype=BF), ht=E(3, 24), chunks=E(1, 3, 24))
+             out=E(1, 130, 24, dtype=BF), ht=E(3, 24), chunks=E(1, 2, 24))
     return scan(**{**a, **over})
 
 
@@ -111,20 +111,20 @@ def test_scan_accepts():
     (scan, dict(out=E(2, 130, 24)), "BAD_DTYPE"), (scan, dict(h0=E(2, 24, dtype=BF)), "BAD_DTYPE"),
     (scan, dict(ht=E(2, 24, dtype=BF)), "BAD_DTYPE"), (packed, dict(cu=E(4, dtype=I32)), "BAD_DTYPE"),
     (scan, dict(g=E(2, 130, 1)), "BAD_SHAPE"), (scan, dict(h0=E(1, 24)), "BAD_SHAPE"),
-    (scan, dict(out=E(2, 129, 24, dtype=BF)), "BAD_SHAPE"), (scan, dict(chunks=E(2, 2, 24)), "BAD_SHAPE"),
+    (scan, dict(out=E(2, 129, 24, dtype=BF)), "BAD_SHAPE"), (scan, dict(chunks=E(2, 3, 24)), "BAD_SHAPE"),
     (scan, dict(x=E(2, 0, 24, dtype=BF)), "NULL_ARGUMENT"),
     (packed, dict(h0=E(4, 24)), "BAD_SHAPE"), (packed, dict(ht=E(2, 24)), "BAD_SHAPE"),
     (scan, dict(cu=E(3, dtype=I64)), "BAD_VARLEN"), (packed, dict(cu=E(1, dtype=I64)), "BAD_VARLEN"),
     (scan, dict(g=E(2, 130, 1).expand(2, 130, 24)), "BAD_STRIDE"),
     (scan, dict(x=E(2, 130, 48, dtype=BF)[..., ::2]), "BAD_STRIDE"),
-    (packed, dict(cu=E(8, dtype=I64)[::2]), "BAD_STRIDE"), (scan, dict(chunks=E(2, 3, 48)[..., :24]), "BAD_STRIDE"),
+    (packed, dict(cu=E(8, dtype=I64)[::2]), "BAD_STRIDE"), (scan, dict(chunks=E(2, 2, 48)[..., :24]), "BAD_STRIDE"),
 ])
 def test_scan_refuses(call, over, status):
     assert name(call(**over)) == status, _lib.last_error()
 
 
 def scan_backward(**over):
-    a = dict(x=E(2, 130, 24, dtype=BF), g=E(2, 130, 24), h0=E(2, 24), cu=None, chunks=E(2, 3, 24),
+    a = dict(x=E(2, 130, 24, dtype=BF), g=E(2, 130, 24), h0=E(2, 24), cu=None, chunks=E(2, 2, 24),
              d_out=E(2, 130, 24, dtype=BF), d_ht=E(2, 24), dx=E(2, 130, 24, dtype=BF), dg=E(2, 130, 24), dh0=E(2, 24))
     a.update(over)
     return _lib.load().cgdrGatedLinearRecurrenceBackward(
