@@ -127,8 +127,9 @@ __device__ __forceinline__ Vec<V> vec_exp(Vec<V> g)
 struct ScanBorders {
     int64_t first, last;  // tokens [first, last) belong to sequences
     int64_t ahead;
+    int64_t sequence;
     __device__ __forceinline__ ScanBorders(const ScanParams& p, bool reverse)
-        : first(0), last(p.T), ahead(reverse ? INT64_MAX : INT64_MIN)
+        : first(0), last(p.T), ahead(reverse ? INT64_MAX : INT64_MIN), sequence(0)
     {
         if (p.cu) {
             first = p.cu[0];
@@ -136,24 +137,40 @@ struct ScanBorders {
             last = end < p.T ? end : p.T;
         }
     }
-    // Bit i: a sequence begins or ends before token t + i, 0 <= i <= 16.
+    // Bit i: a sequence begins or ends before token t + i, 0 <= i <= 16.  Where
+    // there is one, lane i holds the sequence of token t + i afterwards: the
+    // last one that begins at or before it.
     template <bool REVERSE>
-    __device__ __forceinline__ uint32_t at(const ScanParams& p, int64_t t)
+    __device__ __forceinline__ uint32_t at(const ScanParams& p, int64_t b, int64_t t)
     {
         if (REVERSE ? ahead < t : ahead > t + kScanSteps) return 0;
+        const int lane = threadIdx.x % 32;
         uint32_t bits = 0;
+        int begun = 0;                // sequences that begin at or before token t + lane
         unsigned near = 0xffffffffu;  // distance of the nearest border past the 17 places
         const int64_t n = p.cu ? p.N : 1;
-        for (int64_t i = threadIdx.x % 32; i <= n; i += 32) {
-            const int64_t d = (p.cu ? p.cu[i] : i ? p.T : 0) - t;
-            if (d >= 0 && d <= kScanSteps) bits |= 1u << d;
+        for (int64_t i0 = 0; i0 <= n; i0 += 32) {
+            const int64_t i = i0 + lane;
+            const int64_t d = i <= n ? (p.cu ? p.cu[i] : i ? p.T : 0) - t : INT64_MAX;
+            const bool here = d >= 0 && d <= kScanSteps;
+            if (here) bits |= 1u << d;
             const int64_t far = REVERSE ? -d : d - kScanSteps;
             if (far > 0 && far < near) near = static_cast<unsigned>(far);
+            begun += __popc(__ballot_sync(~0u, d < 0));
+            if (__any_sync(~0u, here))
+#pragma unroll 1
+                for (int j = 0; j <= kScanSteps; ++j) {
+                    const int add = __popc(__ballot_sync(~0u, here && d <= j));
+                    if (lane == j) begun += add;
+                }
         }
         near = __reduce_min_sync(~0u, near);
         ahead = REVERSE ? t - near : t + kScanSteps + near;
+        const int64_t s = p.cu ? static_cast<int64_t>(begun) - 1 : b;
+        sequence = s < 0 ? 0 : s < p.N ? s : p.N - 1;
         return __reduce_or_sync(~0u, bits);
     }
+    __device__ __forceinline__ int64_t of(int l) const { return __shfl_sync(~0u, sequence, l); }
     // Bit i: token t + i belongs to no sequence.
     __device__ __forceinline__ uint32_t dead(int64_t t) const
     {
@@ -164,16 +181,6 @@ struct ScanBorders {
         return (before | ~upto) & all;
     }
 };
-
-// The sequence of token t: the last one that begins at or before it.
-__device__ __forceinline__ int64_t scan_sequence(const ScanParams& p, int64_t b, int64_t t)
-{
-    if (!p.cu) return b;
-    unsigned before = 0;
-    for (int64_t i = threadIdx.x % 32; i <= p.N; i += 32) before += p.cu[i] <= t;
-    const int64_t n = static_cast<int64_t>(__reduce_add_sync(~0u, before)) - 1;
-    return n < 0 ? 0 : n < p.N ? n : p.N - 1;
-}
 
 // Channels c .. c + V of row n of a [N, D] fp32 tensor (zeros without one).
 template <int V>
@@ -192,21 +199,6 @@ __device__ __forceinline__ void scan_store_state(float* base, int64_t stride, in
     if (!base || !mine) return;
 #pragma unroll
     for (int i = 0; i < V; ++i) base[n * stride + c + i] = v.v[i];
-}
-
-// The same for the sequence of token t; kept out of line, since few warps meet
-// a border.
-template <int V>
-__device__ __noinline__ Vec<V> scan_load_of(const ScanParams& p, const float* base, int64_t stride, int64_t b, int64_t t,
-                                            int64_t c, bool mine)
-{
-    return scan_load_state<V>(base, stride, scan_sequence(p, b, t), c, mine);
-}
-template <int V>
-__device__ __noinline__ void scan_store_of(const ScanParams& p, float* base, int64_t stride, int64_t b, int64_t t,
-                                           int64_t c, bool mine, Vec<V> v)
-{
-    scan_store_state<V>(base, stride, scan_sequence(p, b, t), c, mine, v);
 }
 
 // States of empty sequences pass through (`to` from `from`).
@@ -646,7 +638,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W)
     for (int seg = 0; seg < segments; ++seg) {
         const int turn = seg & 1;
         const int64_t t = first_token(seg);
-        const uint32_t borders = seqs.at<false>(p, t), dead = seqs.dead(t);
+        const uint32_t borders = seqs.at<false>(p, b, t), dead = seqs.dead(t);
         const bool plain = (borders | dead) == 0;
         const bool there = flight.wait(warp, seg);
         const uint8_t *const px = piece(seg), *const pg = px + RX::kBytes;
@@ -672,7 +664,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W)
                     x[l] = Vec<V>::of(0.0f);
                     m.restart(x[l]);
                 } else if (borders >> l & 1) {
-                    m.restart(scan_load_of<V>(p, p.h0, p.h0_sn, b, t + l, c, mine));
+                    m.restart(scan_load_state<V>(p.h0, p.h0_sn, seqs.of(l), c, mine));
                 }
                 m.a = m.a * a[l];
                 m.b = vec_fma(a[l], m.b, x[l]);
@@ -707,11 +699,11 @@ __global__ void __launch_bounds__(W * 32, 16 / W)
             for (int l = 0; l < kScanSteps; ++l) {
                 const bool out_of = dead >> l & 1;
                 if (out_of) h = Vec<V>::of(0.0f);
-                else if (borders >> l & 1) h = scan_load_of<V>(p, p.h0, p.h0_sn, b, t + l, c, mine);
+                else if (borders >> l & 1) h = scan_load_state<V>(p.h0, p.h0_sn, seqs.of(l), c, mine);
                 h = vec_fma(a[l], h, x[l]);
                 if (t + l < p.T) to.put(l, h);
                 if (!out_of && p.ht && (borders >> (l + 1) & 1))
-                    scan_store_of<V>(p, p.ht, p.ht_sn, b, t + l, c, mine, h);
+                    scan_store_state<V>(p.ht, p.ht_sn, seqs.of(l), c, mine, h);
             }
         }
     }
@@ -794,7 +786,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W)
     for (int k = 0; k < segments; ++k) {
         const int turn = k & 1;
         const int64_t t = first_token(k);
-        const uint32_t borders = seqs.at<true>(p, t), dead = seqs.dead(t);
+        const uint32_t borders = seqs.at<true>(p, b, t), dead = seqs.dead(t);
         const bool plain = (borders | dead) == 0;
         const int64_t chunk = t / kScanChunk;
         Vec<V> h = scan_load_state<V>(p.chunk, p.D, b * chunks + chunk, c, mine && chunk < chunks);  // before this CTA's tokens
@@ -829,13 +821,13 @@ __global__ void __launch_bounds__(W * 32, 16 / W)
                     mu.cut = true;
                     continue;
                 }
-                if (borders >> l & 1) mh.restart(scan_load_of<V>(p, p.h0, p.h0_sn, b, t + l, c, mine));
+                if (borders >> l & 1) mh.restart(scan_load_state<V>(p.h0, p.h0_sn, seqs.of(l), c, mine));
                 mh.a = mh.a * a[l];
                 mh.b = vec_fma(a[l], mh.b, get_x(l));
                 if (!mu.cut) {  // what lies right of the first sequence's end does not reach out
                     mu.b = vec_fma(mh.a, get_d(l), mu.b);
                     if (borders >> (l + 1) & 1) {
-                        mu.b = vec_fma(mh.a, scan_load_of<V>(p, p.d_ht, p.dht_sn, b, t + l, c, mine), mu.b);
+                        mu.b = vec_fma(mh.a, scan_load_state<V>(p.d_ht, p.dht_sn, seqs.of(l), c, mine), mu.b);
                         mu.cut = true;
                     }
                 }
@@ -880,7 +872,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W)
             for (int l = 0; l < kScanSteps; ++l) {
                 before[l] = h;
                 if (dead >> l & 1) continue;
-                if (borders >> l & 1) before[l] = scan_load_of<V>(p, p.h0, p.h0_sn, b, t + l, c, mine);
+                if (borders >> l & 1) before[l] = scan_load_state<V>(p.h0, p.h0_sn, seqs.of(l), c, mine);
                 h = vec_fma(a[l], before[l], get_x(l));
             }
 #pragma unroll
@@ -889,12 +881,12 @@ __global__ void __launch_bounds__(W * 32, 16 / W)
                 if (dead >> l & 1) {
                     u = dh;
                 } else {
-                    if (borders >> (l + 1) & 1) u = scan_load_of<V>(p, p.d_ht, p.dht_sn, b, t + l, c, mine);
+                    if (borders >> (l + 1) & 1) u = scan_load_state<V>(p.d_ht, p.dht_sn, seqs.of(l), c, mine);
                     dh = u + get_d(l);
                     u = a[l] * dh;
                     dgv = u * before[l];
                     if (p.d_h0 && (borders >> l & 1))
-                        scan_store_of<V>(p, p.d_h0, p.dh0_sn, b, t + l, c, mine, u);
+                        scan_store_state<V>(p.d_h0, p.dh0_sn, seqs.of(l), c, mine, u);
                 }
                 if (t + l < p.T) {
                     to_x.put(l, dh);
