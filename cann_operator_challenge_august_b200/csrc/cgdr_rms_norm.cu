@@ -60,44 +60,52 @@ cgdrStatus check_x(const cgdrTensor* x, const cgdrTensor* weight, const char* na
     return check_inner_contiguous(weight, "weight");
 }
 
-// Calls f.template operator()<TX, LPR, NV>() for x's type and row length: the
-// fewest lanes that hold a row in four pieces a lane, and one piece a lane
-// where a row fits a warp.
+// Calls f.template operator()<TX, V, LPR, NV>() for x's type and row length.
+// Pieces of 16 bytes: the fewest lanes that hold a row in four pieces a lane
+// (`most`; a lane of a longer row has eight, and one piece where a row fits a
+// warp).  Single columns where rows are not made of such pieces.
 template <typename TX, typename F>
-void with_shape(int64_t D, F& f)
+void with_shape(int64_t D, bool pieces, F& f)
 {
     constexpr int V = 16 / sizeof(TX);
-    const int64_t pieces = (D + V - 1) / V;
-    if (pieces <= 8) f.template operator()<TX, 8, 1>();
-    else if (pieces <= 16) f.template operator()<TX, 16, 1>();
-    else if (pieces <= 32) f.template operator()<TX, 32, 1>();
-    else if (pieces <= 64) f.template operator()<TX, 32, 2>();
-    else if (pieces <= 128) f.template operator()<TX, 32, 4>();
-    else if (pieces <= 256) f.template operator()<TX, 128, 2>();
-    else if (pieces <= 512) f.template operator()<TX, 256, 2>();
-    else if (pieces <= 1024) f.template operator()<TX, 256, 4>();
-    else if (pieces <= 2048) f.template operator()<TX, 512, 4>();
-    else if constexpr (V == 4) f.template operator()<TX, 1024, 4>();
+    if (!pieces) {
+        if (D <= 128) f.template operator()<TX, 1, 32, 4>();
+        else if (D <= 1024) f.template operator()<TX, 1, 256, 4>();
+        else if (D <= 4096) f.template operator()<TX, 1, 512, 8>();
+        else f.template operator()<TX, 1, 1024, 16>();
+        return;
+    }
+    const int64_t n = (D + V - 1) / V;
+    if (n <= 8) f.template operator()<TX, V, 8, 1>();
+    else if (n <= 16) f.template operator()<TX, V, 16, 1>();
+    else if (n <= 32) f.template operator()<TX, V, 32, 1>();
+    else if (n <= 64) f.template operator()<TX, V, 32, 2>();
+    else if (n <= 128) f.template operator()<TX, V, 64, 2>();
+    else if (n <= 256) f.template operator()<TX, V, 128, 2>();
+    else if (n <= 512) f.template operator()<TX, V, 256, 2>();
+    else if (n <= 1024) f.template operator()<TX, V, 512, 2>();
+    else if (n <= 2048) f.template operator()<TX, V, 1024, 2>();
+    else if constexpr (V == 4) f.template operator()<TX, V, 1024, 4>();
 }
 
 template <typename F>
-void with_type(int32_t dt, int64_t D, F&& f)
+void with_type(int32_t dt, int64_t D, bool pieces, F&& f)
 {
-    if (dt == CGDR_DT_BF16) with_shape<__nv_bfloat16>(D, f);
-    else if (dt == CGDR_DT_FLOAT16) with_shape<__half>(D, f);
-    else with_shape<float>(D, f);
+    if (dt == CGDR_DT_BF16) with_shape<__nv_bfloat16>(D, pieces, f);
+    else if (dt == CGDR_DT_FLOAT16) with_shape<__half>(D, pieces, f);
+    else with_shape<float>(D, pieces, f);
 }
 
 struct LaunchForward {
     const NormParams& p;
     bool fp8;
     cudaStream_t stream;
-    template <typename TX, int LPR, int NV>
+    template <typename TX, int V, int LPR, int NV>
     void operator()()
     {
         const unsigned grid = static_cast<unsigned>((p.R + norm_rows(LPR) - 1) / norm_rows(LPR));
-        if (fp8) norm_forward_kernel<TX, LPR, NV, true><<<grid, norm_threads(LPR), 0, stream>>>(p);
-        else norm_forward_kernel<TX, LPR, NV, false><<<grid, norm_threads(LPR), 0, stream>>>(p);
+        if (fp8) norm_forward_kernel<TX, V, LPR, NV, true><<<grid, norm_threads(LPR), 0, stream>>>(p);
+        else norm_forward_kernel<TX, V, LPR, NV, false><<<grid, norm_threads(LPR), 0, stream>>>(p);
     }
 };
 
@@ -105,12 +113,14 @@ struct LaunchBackward {
     const NormBackwardParams& p;
     cudaStream_t stream;
     int64_t grid = 0;
-    template <typename TX, int LPR, int NV>
+    template <typename TX, int V, int LPR, int NV>
     void operator()()
     {
         grid = (p.R + norm_rows(LPR) - 1) / norm_rows(LPR);
         if (grid > kBackwardBlocks) grid = kBackwardBlocks;
-        norm_backward_kernel<TX, LPR, NV><<<static_cast<unsigned>(grid), norm_threads(LPR), 0, stream>>>(p);
+        const unsigned n = static_cast<unsigned>(grid);
+        if (p.gate) norm_backward_kernel<TX, V, LPR, NV, true><<<n, norm_threads(LPR), 0, stream>>>(p);
+        else norm_backward_kernel<TX, V, LPR, NV, false><<<n, norm_threads(LPR), 0, stream>>>(p);
     }
 };
 
@@ -168,7 +178,7 @@ cgdrStatus cgdrRmsNorm(const cgdrTensor* x, const cgdrTensor* weight, const cgdr
         if ((y_scale->shape[1] > 1 && y_scale->strides[1] != 1) || (R > 1 && y_scale->strides[0] != D / group))
             return fail(CGDR_STATUS_BAD_STRIDE, "y_scale must be contiguous");
         p.scale = static_cast<float*>(y_scale->data);
-        p.group_lanes = group == D ? 0 : static_cast<int32_t>(group / V);
+        p.group = static_cast<int32_t>(group);
     }
     p.x = x->data; p.x_s = x->strides[0];
     p.w = weight->data; p.w_f32 = weight->dtype == CGDR_DT_FLOAT32;
@@ -179,9 +189,9 @@ cgdrStatus cgdrRmsNorm(const cgdrTensor* x, const cgdrTensor* weight, const cgdr
     }
     if (present(gate)) { p.gate = gate->data; p.a_s = gate->strides[0]; }
     p.R = R; p.D = D; p.eps = static_cast<float>(eps);
-    p.aligned = pieces_aligned(x, V) && pieces_aligned(weight, V) && pieces_aligned(residual, V) &&
-                pieces_aligned(gate, V) && pieces_aligned(y, V) && pieces_aligned(z, V);
-    with_type(x->dtype, D, LaunchForward{p, fp8, static_cast<cudaStream_t>(stream)});
+    const bool pieces = pieces_aligned(x, V) && pieces_aligned(weight, V) && pieces_aligned(residual, V) &&
+                        pieces_aligned(gate, V) && pieces_aligned(y, V) && pieces_aligned(z, V);
+    with_type(x->dtype, D, pieces, LaunchForward{p, fp8, static_cast<cudaStream_t>(stream)});
     return launched("rms norm");
 }
 
@@ -235,10 +245,10 @@ cgdrStatus cgdrRmsNormBackward(const cgdrTensor* z, const cgdrTensor* weight, co
     if (present(dgate)) { p.dgate = dgate->data; p.da_s = dgate->strides[0]; }
     p.R = R; p.D = D; p.eps = static_cast<float>(eps);
     const int64_t V = 16 / bytes_of(z->dtype);
-    p.aligned = pieces_aligned(weight, V);
-    for (const cgdrTensor* t : {z, gate, dy, dz, dx, dgate}) p.aligned = p.aligned && pieces_aligned(t, V);
+    bool pieces = pieces_aligned(weight, V);
+    for (const cgdrTensor* t : {z, gate, dy, dz, dx, dgate}) pieces = pieces && pieces_aligned(t, V);
     LaunchBackward launch{p, stream};
-    with_type(z->dtype, D, launch);
+    with_type(z->dtype, D, pieces, launch);
     if ((st = launched("rms norm, backward"))) return st;
     if (p.dw) {
         if (dweight->dtype == CGDR_DT_FLOAT32) sum_weight<float>(p, launch.grid, dweight, stream);

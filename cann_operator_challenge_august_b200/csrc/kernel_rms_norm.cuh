@@ -15,8 +15,8 @@ struct NormParams {
     void *y, *z;
     float* scale;  // 8-bit output: one per group
     int64_t R, D, x_s, r_s, a_s, y_s, z_s;
-    int32_t group_lanes;  // lanes that share a scale; 0: the whole row
-    int32_t w_f32, aligned;
+    int32_t group;  // columns that share a scale
+    int32_t w_f32;
     float eps;
 };
 
@@ -25,38 +25,24 @@ struct NormBackwardParams {
     void *dx, *dgate;                    // may be nullptr
     float* dw;                           // partial sums [gridDim.x, D]; nullptr: not wanted
     int64_t R, D, z_s, a_s, dy_s, dz_s, dx_s, da_s;
-    int32_t w_f32, aligned;
+    int32_t w_f32;
     float eps;
 };
 
+// weight[c .. c + V) as fp32
 template <typename T, int V>
-__device__ __forceinline__ Pack<T, V> norm_load(const T* p, int32_t aligned, int valid)
-{
-    return aligned ? load_pack<T, V, true>(p) : load_pack<T, V, false>(p, valid);
-}
-
-template <typename T, int V>
-__device__ __forceinline__ void norm_store(T* p, const float* v, int32_t aligned, int valid)
-{
-    if (aligned) store_pack<T, V, true>(p, v);
-    else store_pack<T, V, false>(p, v, valid);
-}
-
-// weight[c .. c + V) as fp32 (the address of `w` is checked with the rows')
-template <typename T, int V>
-__device__ __forceinline__ void norm_weight(const void* w, int32_t w_f32, int32_t aligned, int64_t c, int valid,
-                                            float* out)
+__device__ __forceinline__ void norm_weight(const void* w, int32_t w_f32, int64_t c, float* out)
 {
     if (w_f32) {
-        const float* const f = static_cast<const float*>(w) + c;
+        constexpr int F = V < 4 ? V : 4;
 #pragma unroll
-        for (int i = 0; i < V; i += 4) {
-            const auto pk = norm_load<float, 4>(f + i, aligned, valid - i);
+        for (int i = 0; i < V; i += F) {
+            const auto pk = load_pack<float, F, true>(static_cast<const float*>(w) + c + i);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) out[i + k] = pk.e[k];
+            for (int k = 0; k < F; ++k) out[i + k] = pk.e[k];
         }
     } else {
-        const auto pk = norm_load<T, V>(static_cast<const T*>(w) + c, aligned, valid);
+        const auto pk = load_pack<T, V, true>(static_cast<const T*>(w) + c);
 #pragma unroll
         for (int i = 0; i < V; ++i) out[i] = to_f32(pk.e[i]);
     }
@@ -73,135 +59,175 @@ __device__ __forceinline__ float max_nan(float a, float b)
     return r;
 }
 
-// Sums (or NaN-keeping maxima) over the LPR lanes of a row: shuffles inside a
-// warp, then shared memory where a row spans the block.  `slot` tells two
-// reductions of one row apart.
-template <int LPR, bool MAX>
-__device__ __forceinline__ float row_reduce(float v, float (*shared)[32], int slot)
-{
-#pragma unroll
-    for (int m = (LPR < 32 ? LPR : 32) / 2; m > 0; m >>= 1) {
-        const float o = __shfl_xor_sync(~0u, v, m);
-        v = MAX ? max_nan(v, o) : v + o;
-    }
-    if constexpr (LPR > 32) {
-        constexpr int W = LPR / 32;
-        if (threadIdx.x % 32 == 0) shared[slot][threadIdx.x / 32] = v;
-        __syncthreads();
-        v = shared[slot][0];
-#pragma unroll
-        for (int i = 1; i < W; ++i) v = MAX ? max_nan(v, shared[slot][i]) : v + shared[slot][i];
-    }
-    return v;
-}
-
 constexpr int norm_threads(int lpr) { return lpr <= 32 ? 256 : lpr; }
 constexpr int norm_rows(int lpr) { return lpr <= 32 ? 256 / lpr : 1; }
 
-// LPR lanes share a row and hold it in registers, NV pieces of 16 bytes each,
-// so every input is read once and every output written once: the kernel is
-// bound by DRAM.  Piece j of lane l holds columns (j LPR + l) V .. + V.
-template <typename TX, int LPR, int NV, bool FP8>
+// Sums of N values (or NaN-keeping maxima) over the LPR lanes of a row:
+// shuffles inside a warp, then `shared` where a row spans the block.  Two
+// reductions that follow one another use different parts of it.
+template <int LPR, bool MAX, int N>
+__device__ __forceinline__ void row_reduce(float (&v)[N], float (*shared)[32])
+{
+#pragma unroll
+    for (int m = (LPR < 32 ? LPR : 32) / 2; m > 0; m >>= 1)
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const float o = __shfl_xor_sync(~0u, v[k], m);
+            v[k] = MAX ? max_nan(v[k], o) : v[k] + o;
+        }
+    if constexpr (LPR > 32) {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (threadIdx.x % 32 == 0) shared[k][threadIdx.x / 32] = v[k];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            v[k] = shared[k][0];
+#pragma unroll
+            for (int i = 1; i < LPR / 32; ++i) v[k] = MAX ? max_nan(v[k], shared[k][i]) : v[k] + shared[k][i];
+        }
+    }
+}
+
+// scale of a group whose largest |y| is `amax`; the clamp keeps a NaN
+__device__ __forceinline__ float norm_scale(float amax) { return (amax < 1e-12f ? 1e-12f : amax) * (1.0f / 448.0f); }
+
+// Four values of a row as e4m3, to the nearest, saturating.
+template <int V>
+__device__ __forceinline__ void norm_store_fp8(uint8_t* to, const float* v)
+{
+    alignas(8) uint8_t q[V];
+    if constexpr (V == 1) {
+        q[0] = __nv_cvt_float_to_fp8(v[0], __NV_SATFINITE, __NV_E4M3);
+        *to = q[0];
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i += 2)
+            *reinterpret_cast<__nv_fp8x2_storage_t*>(q + i) =
+                __nv_cvt_float2_to_fp8x2(make_float2(v[i], v[i + 1]), __NV_SATFINITE, __NV_E4M3);
+        using Raw = typename RawOf<V>::type;
+        *reinterpret_cast<Raw*>(to) = *reinterpret_cast<const Raw*>(q);
+    }
+}
+
+// LPR lanes share a row and hold it in registers, NV pieces of V columns each
+// (16 bytes; one column where rows are not made of 16-byte pieces), so every
+// input is read once and every output written once: the kernel is bound by
+// DRAM.  Piece j of lane l holds columns (j LPR + l) V .. + V.  All loads of a
+// row are issued before anything waits for one.  z is kept as it is stored,
+// in its own type.
+template <typename TX, int V, int LPR, int NV, bool FP8>
 __global__ void __launch_bounds__(norm_threads(LPR)) norm_forward_kernel(const NormParams p)
 {
-    constexpr int V = 16 / sizeof(TX);
-    __shared__ float shared[2][32];
-    const int lane = threadIdx.x % LPR;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * norm_rows(LPR) + threadIdx.x / LPR;
+    __shared__ float shared[2][1][32];
+    // with one column a lane a group spans warps: its maximum, as the ordered
+    // bits of a value that is not negative
+    constexpr int kGroups = FP8 && V == 1 ? (LPR * NV + 31) / 32 : 1;
+    __shared__ unsigned group_max[norm_rows(LPR)][kGroups];
+    const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * norm_rows(LPR) + sub;
     const bool in = row < p.R;
-    float z[NV][V];
-    Pack<TX, V> gate[NV];
-    float ss = 0.0f;
+    const int64_t D = in ? p.D : 0;
+    Pack<TX, V> z[NV], r[NV], gate[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int64_t c = static_cast<int64_t>(j * LPR + lane) * V;
-        const int valid = static_cast<int>(p.D - c);
-        if (in && valid > 0) {
-            const auto x = norm_load<TX, V>(static_cast<const TX*>(p.x) + row * p.x_s + c, p.aligned, valid);
-            if (p.gate)
-                gate[j] = norm_load<TX, V>(static_cast<const TX*>(p.gate) + row * p.a_s + c, p.aligned, valid);
-            if (p.residual) {
-                const auto r = norm_load<TX, V>(static_cast<const TX*>(p.residual) + row * p.r_s + c, p.aligned, valid);
-#pragma unroll
-                for (int i = 0; i < V; ++i) z[j][i] = to_f32(from_f32<TX>(to_f32(x.e[i]) + to_f32(r.e[i])));
-                norm_store<TX, V>(static_cast<TX*>(p.z) + row * p.z_s + c, z[j], p.aligned, valid);
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i) z[j][i] = to_f32(x.e[i]);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                z[j][i] = 0.0f;
-                gate[j].e[i] = from_f32<TX>(0.0f);
-            }
+        z[j] = r[j] = gate[j] = pack_zero<TX, V>();
+        if (c < D) {
+            z[j] = load_pack<TX, V, true>(static_cast<const TX*>(p.x) + row * p.x_s + c);
+            if (p.residual) r[j] = load_pack<TX, V, true>(static_cast<const TX*>(p.residual) + row * p.r_s + c);
+            if (p.gate) gate[j] = load_pack<TX, V, true>(static_cast<const TX*>(p.gate) + row * p.a_s + c);
         }
-#pragma unroll
-        for (int i = 0; i < V; ++i) ss = fmaf(z[j][i], z[j][i], ss);
     }
-    ss = row_reduce<LPR, false>(ss, shared, 0);
-    const float r = rsqrtf(ss / static_cast<float>(p.D) + p.eps);
-    float amax = 0.0f;
+    if (p.residual) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t c = static_cast<int64_t>(j * LPR + lane) * V;
+            float f[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = to_f32(z[j].e[i]) + to_f32(r[j].e[i]);
+            z[j] = to_pack<TX, V>(f);
+            if (c < D) *reinterpret_cast<Pack<TX, V>*>(static_cast<TX*>(p.z) + row * p.z_s + c) = z[j];
+        }
+    }
+    float ss[1] = {0.0f};
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) ss[0] = fmaf(to_f32(z[j].e[i]), to_f32(z[j].e[i]), ss[0]);
+    if constexpr (FP8 && V == 1) {
+        for (int i = threadIdx.x; i < norm_rows(LPR) * kGroups; i += blockDim.x) (&group_max[0][0])[i] = 0;
+        __syncthreads();
+    }
+    row_reduce<LPR, false>(ss, shared[0]);
+    const float inv_rms = rsqrtf(ss[0] / static_cast<float>(p.D) + p.eps);
+
+    float y[FP8 ? NV : 1][V];
+    float amax[1] = {0.0f};
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int64_t c = static_cast<int64_t>(j * LPR + lane) * V;
-        const int valid = static_cast<int>(p.D - c);
-        if (in && valid > 0) {
-            float w[V];
-            norm_weight<TX, V>(p.w, p.w_f32, p.aligned, c, valid, w);
+        float* const v = y[FP8 ? j : 0];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                z[j][i] *= r * w[i];
-                if (p.gate) {
+        for (int i = 0; i < V; ++i) v[i] = 0.0f;
+        if (c < D) {
+            float w[V];
+            norm_weight<TX, V>(p.w, p.w_f32, c, w);
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = to_f32(z[j].e[i]) * (inv_rms * w[i]);
+            if (p.gate) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
                     const float a = to_f32(gate[j].e[i]);
-                    z[j][i] *= a * sigmoid_fast(a);
+                    v[i] *= a * sigmoid_fast(a);
                 }
-                if constexpr (FP8) amax = max_nan(amax, fabsf(z[j][i]));
             }
-            if constexpr (!FP8) norm_store<TX, V>(static_cast<TX*>(p.y) + row * p.y_s + c, z[j], p.aligned, valid);
+            if constexpr (!FP8) store_pack<TX, V, true>(static_cast<TX*>(p.y) + row * p.y_s + c, v);
         }
         if constexpr (FP8) {
-            if (p.group_lanes) {  // uniform: a scale for each group of lanes of this piece
-                for (int m = p.group_lanes / 2; m > 0; m >>= 1) amax = max_nan(amax, __shfl_xor_sync(~0u, amax, m));
-                // the clamp keeps a NaN
-                const float scale = (amax < 1e-12f ? 1e-12f : amax) * (1.0f / 448.0f);
-                if (in && valid > 0) {
+            float most = 0.0f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) most = max_nan(most, fabsf(v[i]));
+            if (p.group == p.D) {
+                amax[0] = max_nan(amax[0], most);
+            } else if constexpr (V == 1) {
+                if (c < D) atomicMax(&group_max[sub][c / p.group], __float_as_uint(most));
+            } else {  // a group lies in neighbouring lanes of one piece
+                const int lanes = p.group / V;
+                for (int m = lanes / 2; m > 0; m >>= 1) most = max_nan(most, __shfl_xor_sync(~0u, most, m));
+                const float scale = norm_scale(most);
+                if (c < D) {
                     const float inv = 1.0f / scale;
 #pragma unroll
-                    for (int i = 0; i < V; ++i) z[j][i] *= inv;
-                    if (lane % p.group_lanes == 0) p.scale[(row * p.D + c) / (p.group_lanes * V)] = scale;
+                    for (int i = 0; i < V; ++i) v[i] *= inv;
+                    norm_store_fp8<V>(static_cast<uint8_t*>(p.y) + row * p.y_s + c, v);
+                    if (lane % lanes == 0) p.scale[row * (p.D / p.group) + c / p.group] = scale;
                 }
-                amax = 0.0f;
             }
         }
     }
     if constexpr (FP8) {
-        float inv = 1.0f;
-        if (!p.group_lanes) {
-            amax = row_reduce<LPR, true>(amax, shared, 1);
-            const float scale = (amax < 1e-12f ? 1e-12f : amax) * (1.0f / 448.0f);
-            inv = 1.0f / scale;
+        if (p.group != p.D && V > 1) return;
+        float scale = 0.0f;
+        if (p.group == p.D) {
+            row_reduce<LPR, true>(amax, shared[1]);
+            scale = norm_scale(amax[0]);
             if (in && lane == 0) p.scale[row] = scale;
+        } else {
+            __syncthreads();
         }
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int64_t c = static_cast<int64_t>(j * LPR + lane) * V;
-            const int valid = static_cast<int>(p.D - c);
-            if (!in || valid <= 0) continue;
-            uint8_t* const to = static_cast<uint8_t*>(p.y) + row * p.y_s + c;
-            alignas(8) uint8_t q[V];
-#pragma unroll
-            for (int i = 0; i < V; i += 2)
-                *reinterpret_cast<__nv_fp8x2_storage_t*>(q + i) =
-                    __nv_cvt_float2_to_fp8x2(make_float2(z[j][i] * inv, z[j][i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-            if (p.aligned) {
-                using Raw = typename RawOf<V>::type;
-                *reinterpret_cast<Raw*>(to) = *reinterpret_cast<const Raw*>(q);
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; ++i)
-                    if (i < valid) to[i] = q[i];
+            if (c >= D) continue;
+            if (p.group != p.D) {
+                scale = norm_scale(__uint_as_float(group_max[sub][c / p.group]));
+                if (c % p.group == 0) p.scale[row * (p.D / p.group) + c / p.group] = scale;
             }
+            const float inv = 1.0f / scale;
+#pragma unroll
+            for (int i = 0; i < V; ++i) y[j][i] *= inv;
+            norm_store_fp8<V>(static_cast<uint8_t*>(p.y) + row * p.y_s + c, y[j]);
         }
     }
 }
@@ -209,90 +235,94 @@ __global__ void __launch_bounds__(norm_threads(LPR)) norm_forward_kernel(const N
 // The same split of a row.  With u = dy w silu(gate), both sums of a row are
 // taken in one reduction,
 //     dx = r u - z r^3 mean(u z) + dz,   r = (mean(z^2) + eps)^(-1/2)
-// so r is recomputed from z rather than kept.  Blocks walk over the rows and
-// keep their share of dweight in registers; it leaves the block once, summed
-// over its rows in a fixed order, and a second kernel adds the blocks.
-template <typename TX, int LPR, int NV>
-__global__ void __launch_bounds__(norm_threads(LPR)) norm_backward_kernel(const NormBackwardParams p)
+// so r is recomputed from z rather than kept.  Blocks walk over the rows; a
+// lane's columns stay the same, so the weight and dweight's share live in
+// registers, and the next row's loads are issued before this row's sums are
+// awaited.  dweight leaves a block once, summed over its rows in a fixed
+// order, and a second kernel adds the blocks.
+template <typename TX, int V, int LPR, int NV, bool GATE>
+__global__ void __launch_bounds__(norm_threads(LPR), LPR <= 256 ? 2 : 1)
+    norm_backward_kernel(const NormBackwardParams p)
 {
-    constexpr int V = 16 / sizeof(TX);
     constexpr int G = norm_rows(LPR);
-    __shared__ float shared[4][32];
-    __shared__ float part[G > 1 ? G : 1][G > 1 ? LPR * NV * V : 1];
+    __shared__ float shared[2][2][32];
+    __shared__ float part[G][G > 1 ? LPR * NV * V : 1];
     const int lane = threadIdx.x % LPR, group = threadIdx.x / LPR;
-    float dw[NV][V];
+    const float inv_d = 1.0f / static_cast<float>(p.D);
+    float w[NV][V], dw[NV][V];
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j) {
+        const int64_t c = static_cast<int64_t>(j * LPR + lane) * V;
 #pragma unroll
-        for (int i = 0; i < V; ++i) dw[j][i] = 0.0f;
+        for (int i = 0; i < V; ++i) w[j][i] = dw[j][i] = 0.0f;
+        if (c < p.D) norm_weight<TX, V>(p.w, p.w_f32, c, w[j]);
+    }
+    struct Row {
+        Pack<TX, V> z[NV], dy[NV], gate[GATE ? NV : 1], dz[NV];
+    };
+    auto load = [&](int64_t blk, Row& r) {
+        const int64_t row = blk * G + group;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t c = static_cast<int64_t>(j * LPR + lane) * V;
+            r.z[j] = r.dy[j] = r.dz[j] = r.gate[GATE ? j : 0] = pack_zero<TX, V>();
+            if (row < p.R && c < p.D) {
+                r.z[j] = load_pack<TX, V, true>(static_cast<const TX*>(p.z) + row * p.z_s + c);
+                r.dy[j] = load_pack<TX, V, true>(static_cast<const TX*>(p.dy) + row * p.dy_s + c);
+                if (GATE) r.gate[GATE ? j : 0] = load_pack<TX, V, true>(static_cast<const TX*>(p.gate) + row * p.a_s + c);
+                if (p.dz) r.dz[j] = load_pack<TX, V, true>(static_cast<const TX*>(p.dz) + row * p.dz_s + c);
+            }
+        }
+    };
     const int64_t blocks = (p.R + G - 1) / G;
+    Row now;
+    load(blockIdx.x, now);
     int turn = 0;
-    for (int64_t blk = blockIdx.x; blk < blocks; blk += gridDim.x, turn ^= 2) {
+    for (int64_t blk = blockIdx.x; blk < blocks; blk += gridDim.x, turn ^= 1) {
         const int64_t row = blk * G + group;
         const bool in = row < p.R;
-        Pack<TX, V> z[NV], dy[NV], gate[NV], dz[NV];
-        float ss = 0.0f, su = 0.0f;
+        Row next;
+        load(blk + gridDim.x, next);
+        float sums[2] = {0.0f, 0.0f}, sig[GATE ? NV : 1][V];
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int64_t c = static_cast<int64_t>(j * LPR + lane) * V;
-            const int valid = static_cast<int>(p.D - c);
-            if (in && valid > 0) {
-                z[j] = norm_load<TX, V>(static_cast<const TX*>(p.z) + row * p.z_s + c, p.aligned, valid);
-                dy[j] = norm_load<TX, V>(static_cast<const TX*>(p.dy) + row * p.dy_s + c, p.aligned, valid);
-                if (p.gate)
-                    gate[j] = norm_load<TX, V>(static_cast<const TX*>(p.gate) + row * p.a_s + c, p.aligned, valid);
-                if (p.dz) dz[j] = norm_load<TX, V>(static_cast<const TX*>(p.dz) + row * p.dz_s + c, p.aligned, valid);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int64_t c = static_cast<int64_t>(j * LPR + lane) * V;
-            const int valid = static_cast<int>(p.D - c);
-            if (in && valid > 0) {
-                float w[V];
-                norm_weight<TX, V>(p.w, p.w_f32, p.aligned, c, valid, w);
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float f = to_f32(z[j].e[i]);
-                    float u = to_f32(dy[j].e[i]) * w[i];
-                    if (p.gate) {
-                        const float a = to_f32(gate[j].e[i]);
-                        u *= a * sigmoid_fast(a);
-                    }
-                    ss = fmaf(f, f, ss);
-                    su = fmaf(u, f, su);
-                }
-            }
-        }
-        ss = row_reduce<LPR, false>(ss, shared, turn);
-        su = row_reduce<LPR, false>(su, shared, turn + 1);
-        const float inv_d = 1.0f / static_cast<float>(p.D);
-        const float r = rsqrtf(ss * inv_d + p.eps);
-        const float m = r * r * (su * inv_d);
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int64_t c = static_cast<int64_t>(j * LPR + lane) * V;
-            const int valid = static_cast<int>(p.D - c);
-            if (!in || valid <= 0) continue;
-            float w[V], dx[V], da[V];
-            norm_weight<TX, V>(p.w, p.w_f32, p.aligned, c, valid, w);
+        for (int j = 0; j < NV; ++j)
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float f = to_f32(z[j].e[i]), n = f * r;
-                float d = to_f32(dy[j].e[i]), u = d * w[i];
-                if (p.gate) {
-                    const float a = to_f32(gate[j].e[i]), s = sigmoid_fast(a), act = a * s;
-                    da[i] = u * n * (s + act * (1.0f - s));
-                    u *= act;
+                const float f = to_f32(now.z[j].e[i]);
+                float u = to_f32(now.dy[j].e[i]) * w[j][i];
+                if (GATE) {
+                    const float a = to_f32(now.gate[GATE ? j : 0].e[i]);
+                    sig[GATE ? j : 0][i] = sigmoid_fast(a);
+                    u *= a * sig[GATE ? j : 0][i];
+                }
+                sums[0] = fmaf(f, f, sums[0]);
+                sums[1] = fmaf(u, f, sums[1]);
+            }
+        row_reduce<LPR, false>(sums, shared[turn]);
+        const float r = rsqrtf(sums[0] * inv_d + p.eps);
+        const float m = sums[1] * inv_d * r * r * r;  // in an order that does not underflow
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int64_t c = static_cast<int64_t>(j * LPR + lane) * V;
+            float dx[V], da[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float f = to_f32(now.z[j].e[i]), n = f * r;
+                float d = to_f32(now.dy[j].e[i]);
+                if (GATE) {
+                    const float a = to_f32(now.gate[GATE ? j : 0].e[i]), s = sig[GATE ? j : 0][i], act = a * s;
+                    da[i] = d * w[j][i] * n * fmaf(act, 1.0f - s, s);
                     d *= act;
                 }
                 dw[j][i] = fmaf(d, n, dw[j][i]);
-                dx[i] = r * (u - f * m);
-                if (p.dz) dx[i] += to_f32(dz[j].e[i]);
+                dx[i] = fmaf(r, d * w[j][i], to_f32(now.dz[j].e[i])) - f * m;
             }
-            if (p.dx) norm_store<TX, V>(static_cast<TX*>(p.dx) + row * p.dx_s + c, dx, p.aligned, valid);
-            if (p.dgate) norm_store<TX, V>(static_cast<TX*>(p.dgate) + row * p.da_s + c, da, p.aligned, valid);
+            if (in && c < p.D) {
+                if (p.dx) store_pack<TX, V, true>(static_cast<TX*>(p.dx) + row * p.dx_s + c, dx);
+                if (GATE && p.dgate) store_pack<TX, V, true>(static_cast<TX*>(p.dgate) + row * p.da_s + c, da);
+            }
         }
+        now = next;
     }
     if (!p.dw) return;
     float* const to = p.dw + static_cast<int64_t>(blockIdx.x) * p.D;

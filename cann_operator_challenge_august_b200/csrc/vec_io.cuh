@@ -69,8 +69,8 @@ template <> __device__ __forceinline__ void from_f32x2<__half>(float a, float b,
     *reinterpret_cast<__half2*>(to) = __floats2half2_rn(a, b);
 }
 
-template <typename T, int V, bool ALIGNED>
-__device__ __forceinline__ void store_pack(T* p, const float* v, int valid = V)
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> to_pack(const float* v)
 {
     Pack<T, V> r;
     if constexpr (V % 2 == 0) {
@@ -80,6 +80,13 @@ __device__ __forceinline__ void store_pack(T* p, const float* v, int valid = V)
 #pragma unroll
         for (int i = 0; i < V; ++i) r.e[i] = from_f32<T>(v[i]);
     }
+    return r;
+}
+
+template <typename T, int V, bool ALIGNED>
+__device__ __forceinline__ void store_pack(T* p, const float* v, int valid = V)
+{
+    const Pack<T, V> r = to_pack<T, V>(v);
     if constexpr (ALIGNED) {
         using Raw = typename RawOf<sizeof(T) * V>::type;
         *reinterpret_cast<Raw*>(p) = *reinterpret_cast<const Raw*>(&r);
