@@ -135,17 +135,16 @@ class CgdrFwdHPlan(ctypes.Structure):
         return {name: getattr(self, name) for name, _ in self._fields_}
 
 
-# A cgdrTensor as bytes: struct.pack fills it in about a microsecond, a
+# A cgdrTensor as bytes: struct.pack fills it in half a microsecond, a
 # ctypes.Structure field by field in several.  A bytes object passed as
 # char* lends its buffer for the length of the call.
-_VIEW = struct.Struct("@Pii8q8q")
-assert _VIEW.size == ctypes.sizeof(CgdrTensor)
-_ZEROS = tuple((0,) * (MAX_DIMS - n) for n in range(MAX_DIMS + 1))
+_VIEWS = tuple(struct.Struct(f"@Pii{n}q{8 * (MAX_DIMS - n)}x{n}q{8 * (MAX_DIMS - n)}x").pack for n in range(MAX_DIMS + 1))
+assert struct.calcsize("@Pii16q") == ctypes.sizeof(CgdrTensor)
 
 
 def view(data_ptr: int, dtype: int, shape, strides) -> bytes:
-    pad = _ZEROS[len(shape)]
-    return _VIEW.pack(data_ptr, dtype, len(shape), *shape, *pad, *strides, *pad)
+    n = len(shape)
+    return _VIEWS[n](data_ptr, dtype, n, *shape, *strides)
 
 
 _lib = None

@@ -14,12 +14,13 @@ missing.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
 from . import _lib
-from .api import _stream_handle
-from .recurrence import _on_device, _view
+from .api import _DT
+from .recurrence import _new_like, _on_device, _raw_stream, _refuse_twice, _view
 
 
 def _flat(t: torch.Tensor | None, name: str, shape) -> torch.Tensor | None:
@@ -40,28 +41,42 @@ def _flat(t: torch.Tensor | None, name: str, shape) -> torch.Tensor | None:
 
 def _forward(x, weight, eps, residual, gate, group):
     """(y, z or None), or (q, scale, z or None) with a group; all in x's shape."""
+    shape = x.shape
     with _on_device(x, weight, residual, gate):
-        if x.dim() < 1:
+        if not shape:
             raise ValueError("x needs at least one dimension")
-        y = torch.empty(x.shape, dtype=x.dtype if group is None else torch.float8_e4m3fn, device=x.device)
-        z = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        D = shape[-1]
+        z = None if residual is None else _new_like(x)
         scale = None
-        D = x.shape[-1]
-        if group is not None:
+        if group is None:
+            y = _new_like(x)
+        else:
             if group < 1 or D % group:
                 raise ValueError(f"group_size {group} must divide the {D} columns")
-            scale = torch.empty(*x.shape[:-1], D // group, dtype=torch.float32, device=x.device)
+            y = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
+            scale = x.new_empty(*shape[:-1], D // group, dtype=torch.float32)
         if x.numel():
-            shape = x.shape
-            y2 = y if y.dim() == 2 else y.view(-1, D)
+            R = x.numel() // D
+            rows = (R, D), (D, 1)  # the outputs are contiguous
+            dtype = _DT.get(x.dtype, 0)
             st = _lib.load().cgdrRmsNorm(
                 _view(_flat(x, "x", shape)), _view(weight), _view(_flat(residual, "residual", shape)),
-                _view(_flat(gate, "gate", shape)), eps, 0 if group is None else group,
-                _view(y2) if group is None else _lib.view(y.data_ptr(), _lib.DT_FP8_E4M3, y2.shape, y2.stride()),
-                None if scale is None else _view(scale.view(-1, D // group)),
-                None if z is None else _view(z.view(-1, D)), _stream_handle(x.device))
+                _view(_flat(gate, "gate", shape)), eps, group or 0,
+                _lib.view(y.data_ptr(), dtype if group is None else _lib.DT_FP8_E4M3, *rows),
+                None if scale is None else _lib.view(scale.data_ptr(), _lib.DT_FLOAT32, (R, D // group), (D // group, 1)),
+                None if z is None else _lib.view(z.data_ptr(), dtype, *rows), _raw_stream(x.get_device()))
             _lib.check(st, "cgdrRmsNorm")
     return (y, z) if group is None else (y, scale, z)
+
+
+@functools.lru_cache(maxsize=1024)
+def _backward_bytes(R: int, D: int, dtype: int, w_dtype: int) -> int:
+    """Workspace of a backward pass that wants dweight."""
+    size = ctypes.c_uint64(0)
+    st = _lib.load().cgdrRmsNormBackwardGetWorkspaceSize(
+        _lib.view(1, dtype, (R, D), (D, 1)), _lib.view(1, w_dtype, (D,), (1,)), ctypes.byref(size))
+    _lib.check(st, "cgdrRmsNormBackwardGetWorkspaceSize")
+    return size.value
 
 
 class _RmsNorm(torch.autograd.Function):
@@ -74,31 +89,31 @@ class _RmsNorm(torch.autograd.Function):
         return y, z
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dz):
+        _refuse_twice()
         z, weight, gate = ctx.saved_tensors
         want_x, want_w, _, want_r, want_a = ctx.needs_input_grad
         if dy is None:  # z alone was used: its gradient passes through
             return (dz if want_x else None), None, None, (dz if want_r else None), None
-        shape, D = z.shape, z.shape[-1]
+        shape = z.shape
         # gradients arrive with any strides (expanded ones, for a sum)
         dy = dy.contiguous()
         dz = None if dz is None else dz.contiguous()
         with _on_device(z, dy, dz):
-            dx = torch.empty(shape, dtype=z.dtype, device=z.device) if want_x or want_r else None
-            dw = torch.empty(weight.shape, dtype=weight.dtype, device=z.device) if want_w else None
-            da = torch.empty(shape, dtype=z.dtype, device=z.device) if want_a else None
+            dx = _new_like(z) if want_x or want_r else None
+            dw = _new_like(weight) if want_w else None
+            da = _new_like(z) if want_a else None
             if z.numel():
-                lib = _lib.load()
-                flat = lambda t: _view(_flat(t, "gradient", shape))  # noqa: E731
-                z_view, dw_view = flat(z), _view(dw)
-                size = ctypes.c_uint64(0)
-                _lib.check(lib.cgdrRmsNormBackwardGetWorkspaceSize(z_view, dw_view, ctypes.byref(size)),
-                           "cgdrRmsNormBackwardGetWorkspaceSize")
-                ws = torch.empty(size.value, dtype=torch.uint8, device=z.device) if size.value else None
-                st = lib.cgdrRmsNormBackward(
-                    z_view, _view(weight), flat(gate), ctx.eps, flat(dy), flat(dz), flat(dx), dw_view, flat(da),
-                    None if ws is None else ws.data_ptr(), size.value, _stream_handle(z.device))
+                D, dtype = shape[-1], _DT[z.dtype]
+                R = z.numel() // D
+                rows = (R, D), (D, 1)
+                flat = lambda t: None if t is None else _lib.view(t.data_ptr(), dtype, *rows)  # noqa: E731
+                size = _backward_bytes(R, D, dtype, _DT[weight.dtype]) if want_w else 0
+                ws = dy.new_empty(size, dtype=torch.uint8) if size else None
+                st = _lib.load().cgdrRmsNormBackward(
+                    _view(_flat(z, "x", shape)), _view(weight), _view(_flat(gate, "gate", shape)), ctx.eps, flat(dy),
+                    flat(dz), flat(dx), _view(dw), flat(da), None if ws is None else ws.data_ptr(), size,
+                    _raw_stream(z.get_device()))
                 _lib.check(st, "cgdrRmsNormBackward")
             elif dw is not None:
                 dw.zero_()

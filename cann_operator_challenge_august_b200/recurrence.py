@@ -24,26 +24,52 @@ import contextlib
 import torch
 
 from . import _lib
-from .api import _DT, _require_cuda, _stream_handle
+from .api import _DT, _stream_handle
 
 _NO_GUARD = contextlib.nullcontext()
+_VIEWS = _lib._VIEWS
 
 
 def _view(t: torch.Tensor | None) -> bytes | None:
+    """`t` as a cgdrTensor (see _lib.view, inlined: these calls are a short
+    kernel's latency)."""
     if t is None:
         return None
-    return _lib.view(t.data_ptr(), _DT.get(t.dtype, 0), t.shape, t.stride())
+    shape = t.shape
+    n = len(shape)
+    if n > _lib.MAX_DIMS:
+        raise ValueError(f"tensors have at most {_lib.MAX_DIMS} dimensions, got {n}")
+    return _VIEWS[n](t.data_ptr(), _DT.get(t.dtype, 0), n, *shape, *t.stride())
+
+
+# The current stream's handle; the public accessor builds a Stream object first.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: _stream_handle(torch.device("cuda", index)))
 
 
 def _on_device(first: torch.Tensor, *others: torch.Tensor | None):
     """Checks that all tensors are on one CUDA device and returns a context in
     which that device is current."""
-    _require_cuda(first, *others)
-    device = first.device
+    index = first.get_device()
     for t in others:
-        if t is not None and t.device != device:
-            raise ValueError(f"all tensors must be on one device, got {device} and {t.device}")
-    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+        if t is not None and t.get_device() != index:
+            index = -1
+    if index < 0:
+        if all(t is None or t.is_cuda for t in (first, *others)):
+            raise ValueError("all tensors must be on one device")
+        raise ValueError("all tensors must be CUDA tensors (there is no CPU implementation)")
+    return _NO_GUARD if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+def _new_like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _refuse_twice() -> None:
+    """Backward passes call it: gradients are recorded there only for a second
+    derivative, which these operators do not have."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("this operator is differentiable once only")
 
 
 def _updated(state: torch.Tensor) -> None:
@@ -92,12 +118,12 @@ def recurrent_gated_delta_rule(
     raises on that, on indices past the pool and on lengths that do not sum
     to T.  The call is not differentiable."""
     with _on_device(query, key, value, beta, state, actual_seq_lengths, g, state_indices):
-        out = torch.empty(value.shape, dtype=value.dtype, device=value.device)
+        out = _new_like(value)
         status = torch.empty(1, dtype=torch.int32, device=value.device) if check_device_status else None
         st = _lib.load().cgdrRecurrentGatedDeltaRule(
             _view(query), _view(key), _view(value), _view(beta), _view(state), _view(actual_seq_lengths), _view(g),
             _view(state_indices), float(scale if scale is not None else 0.0), _view(out),
-            None if status is None else status.data_ptr(), _stream_handle(value.device))
+            None if status is None else status.data_ptr(), _raw_stream(value.get_device()))
         _lib.check(st, "cgdrRecurrentGatedDeltaRule")
     _updated(state)
     if check_device_status:
@@ -120,11 +146,11 @@ def gated_linear_recurrence_step(
     ``check_device_status`` as in :func:`recurrent_gated_delta_rule`.  The
     call is not differentiable."""
     with _on_device(x, g, state, state_indices):
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = _new_like(x)
         status = torch.empty(1, dtype=torch.int32, device=x.device) if check_device_status else None
         st = _lib.load().cgdrGatedLinearRecurrenceStep(
             _view(x), _view(g), _view(state), _view(state_indices), _view(out),
-            None if status is None else status.data_ptr(), _stream_handle(x.device))
+            None if status is None else status.data_ptr(), _raw_stream(x.get_device()))
         _lib.check(st, "cgdrGatedLinearRecurrenceStep")
     _updated(state)
     if check_device_status:
@@ -135,7 +161,7 @@ def gated_linear_recurrence_step(
 def _forward(x, g, initial_state, cu_seqlens, want_final, want_chunks):
     """(out, final_state or None, chunk_states or None)"""
     with _on_device(x, g, initial_state, cu_seqlens):
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = _new_like(x)
         final = chunks = None
         if x.dim() == 3:  # any other rank is refused by the library
             B, T, D = x.shape
@@ -155,7 +181,7 @@ def _forward(x, g, initial_state, cu_seqlens, want_final, want_chunks):
                 return out, final, chunks
         st = _lib.load().cgdrGatedLinearRecurrence(
             _view(x), _view(g), _view(initial_state), _view(cu_seqlens), _view(out), _view(final), _view(chunks),
-            _stream_handle(x.device))
+            _raw_stream(x.get_device()))
         _lib.check(st, "cgdrGatedLinearRecurrence")
     return out, final, chunks
 
@@ -169,8 +195,8 @@ class _GatedLinearRecurrence(torch.autograd.Function):
         return out, final
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_out, d_final):
+        _refuse_twice()
         x, g, initial_state, cu_seqlens, chunks = ctx.saved_tensors
         if d_out is None and d_final is None:
             return None, None, None, None, None
@@ -179,16 +205,16 @@ class _GatedLinearRecurrence(torch.autograd.Function):
         d_final = None if d_final is None else d_final.contiguous()
         want_x, want_g, want_h0 = ctx.needs_input_grad[:3]
         with _on_device(x, d_out, d_final):
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None
-            dg = torch.empty(g.shape, dtype=g.dtype, device=g.device) if want_g else None
-            dh0 = torch.empty(initial_state.shape, dtype=torch.float32, device=x.device) if want_h0 else None
+            dx = _new_like(x) if want_x else None
+            dg = _new_like(g) if want_g else None
+            dh0 = _new_like(initial_state) if want_h0 else None
             if x.shape[1] == 0:
                 if want_h0:
                     dh0.zero_() if d_final is None else dh0.copy_(d_final)
                 return dx, dg, dh0, None, None
             st = _lib.load().cgdrGatedLinearRecurrenceBackward(
                 _view(x), _view(g), _view(initial_state), _view(cu_seqlens), _view(chunks), _view(d_out),
-                _view(d_final), _view(dx), _view(dg), _view(dh0), _stream_handle(x.device))
+                _view(d_final), _view(dx), _view(dg), _view(dh0), _raw_stream(x.get_device()))
             _lib.check(st, "cgdrGatedLinearRecurrenceBackward")
         return dx, dg, dh0, None, None
 
