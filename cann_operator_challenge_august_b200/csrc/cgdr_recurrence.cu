@@ -98,14 +98,14 @@ void run_delta(DeltaStepParams& p, cudaStream_t stream)
 {
     p.v_tiles = (p.Dv + kDeltaRows * R - 1) / (kDeltaRows * R);
     delta_step_kernel<TX, TS, NV, R, ALIGNED>
-        <<<static_cast<unsigned>(p.B * p.Nv * p.v_tiles), kDeltaThreads, 0, stream>>>(p);
+        <<<p.B * p.Nv * p.v_tiles, kDeltaThreads, 0, stream>>>(p);
 }
 
 template <typename TX, typename TS>
 void dispatch_delta(DeltaStepParams& p, bool aligned, cudaStream_t stream)
 {
     // Two state rows per lane group once that still leaves two CTAs for each SM.
-    const bool wide = p.B * p.Nv * ((p.Dv + 2 * kDeltaRows - 1) / (2 * kDeltaRows)) >= 296;
+    const bool wide = static_cast<int64_t>(p.B) * p.Nv * ((p.Dv + 2 * kDeltaRows - 1) / (2 * kDeltaRows)) >= 296;
     const int nv = p.Dk <= 64 ? 2 : p.Dk <= 128 ? 4 : 8;
     if (!aligned) {
         if (nv == 2) run_delta<TX, TS, 2, 1, false>(p, stream);
@@ -344,14 +344,15 @@ cgdrStatus run_scan(ScanParams& p, const cgdrTensor* x, const cgdrTensor* g, con
 
 struct LaunchStep {
     LinearStepParams& p;
+    unsigned rows;
     bool aligned;
     cudaStream_t stream;
     template <typename TX, typename TG, int V>
     void go()
     {
-        p.tiles = (p.D + kLinearStepThreads * V - 1) / (kLinearStepThreads * V);
+        p.tiles = static_cast<uint32_t>((p.D + kLinearStepThreads * V - 1) / (kLinearStepThreads * V));
         linear_step_kernel<TX, TG, V>
-            <<<static_cast<unsigned>(p.B * p.tiles), kLinearStepThreads, 0, stream>>>(p);
+            <<<rows * p.tiles, kLinearStepThreads, 0, stream>>>(p);
     }
     template <typename TX, typename TG>
     void operator()()
@@ -420,14 +421,16 @@ cgdrStatus cgdrRecurrentGatedDeltaRule(const cgdrTensor* query, const cgdrTensor
         if (!t->data) return fail(CGDR_STATUS_NULL_ARGUMENT, "query, key, value, beta, state and out are required");
     // grid of the narrowest tiles (32 rows)
     const int64_t tiles = (Dv + kDeltaRows - 1) / kDeltaRows;
-    if (B > (int64_t(1) << 31) / Nv || B * Nv >= (int64_t(1) << 31) / tiles)
+    if (Nv >= (int64_t(1) << 31) || B > (int64_t(1) << 31) / Nv || B * Nv >= (int64_t(1) << 31) / tiles)
         return fail(CGDR_STATUS_UNSUPPORTED, "B * Nv * ceil(Dv / 32) must fit in 31 bits");
 
     p.q = query->data; p.k = key->data; p.v = value->data; p.beta = beta->data;
     p.g = has_g ? static_cast<const float*>(g->data) : nullptr;
     p.lens = has_len ? static_cast<const int32_t*>(actual_seq_lengths->data) : nullptr;
     p.state = state->data; p.out = out->data; p.status = device_status;
-    p.B = B; p.T = T; p.Nv = Nv; p.rep = Nv / Nk; p.Dk = Dk; p.Dv = Dv;
+    p.T = T;
+    p.B = static_cast<uint32_t>(B); p.Nv = static_cast<uint32_t>(Nv); p.rep = static_cast<uint32_t>(Nv / Nk);
+    p.Dk = static_cast<uint32_t>(Dk); p.Dv = static_cast<uint32_t>(Dv);
     p.q_st = query->strides[0]; p.q_sh = query->strides[1];
     p.k_st = key->strides[0]; p.k_sh = key->strides[1];
     p.v_st = value->strides[0]; p.v_sh = value->strides[1];
@@ -527,12 +530,12 @@ cgdrStatus cgdrGatedLinearRecurrenceStep(const cgdrTensor* x, const cgdrTensor* 
     if (B >= (int64_t(1) << 31) / tiles) return fail(CGDR_STATUS_UNSUPPORTED, "B * ceil(D / 256) must fit in 31 bits");
     p.x = x->data; p.g = g->data; p.state = static_cast<float*>(state->data); p.out = out->data;
     p.status = device_status;
-    p.B = B; p.D = D;
+    p.D = D;
     p.x_sb = x->strides[0]; p.g_sb = g->strides[0]; p.o_sb = out->strides[0]; p.s_sn = state->strides[0];
     const bool aligned =
         pieces_aligned(x, 4) && pieces_aligned(g, 4) && pieces_aligned(state, 4) && pieces_aligned(out, 4);
     if ((st = clear_status(device_status, stream))) return st;
-    with_types(x->dtype, g->dtype, LaunchStep{p, aligned, stream});
+    with_types(x->dtype, g->dtype, LaunchStep{p, static_cast<unsigned>(B), aligned, stream});
     return launched("gated linear recurrence step");
 }
 

@@ -21,17 +21,17 @@ struct PoolIndex {
     const void* idx;  // nullptr: row b owns state b
     int32_t is64;
     int64_t slots;
-    __device__ __forceinline__ int64_t at(int64_t b) const
+    __device__ __forceinline__ int64_t at(unsigned b) const
     {
         if (!idx) return b;
         return is64 ? static_cast<const int64_t*>(idx)[b] : static_cast<const int32_t*>(idx)[b];
     }
     // whether an earlier row names `slot`, as far as this thread's share goes
-    __device__ __forceinline__ bool seen_before(int64_t b, int64_t slot) const
+    __device__ __forceinline__ bool seen_before(unsigned b, int64_t slot) const
     {
         bool seen = false;
         if (idx && slot >= 0)
-            for (int64_t i = threadIdx.x; i < b; i += blockDim.x) seen |= at(i) == slot;
+            for (unsigned i = threadIdx.x; i < b; i += blockDim.x) seen |= at(i) == slot;
         return seen;
     }
 };
@@ -45,7 +45,8 @@ struct DeltaStepParams {
     void *state, *out;
     int32_t* status;        // nullptr: not reported
     PoolIndex pool;
-    int64_t B, T, Nv, rep, Dk, Dv, v_tiles;
+    int64_t T;
+    uint32_t B, Nv, rep, Dk, Dv, v_tiles;
     int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, o_st, o_sh, b_st, b_sh, g_st, g_sh;
     int64_t s_sn, s_sh, s_sv;
     float scale;
@@ -55,6 +56,9 @@ struct DeltaStepParams {
 constexpr int kDeltaThreads = 256;
 constexpr int kDeltaLanes = 8;                             // lanes that share one state row
 constexpr int kDeltaRows = kDeltaThreads / kDeltaLanes;    // state rows of a CTA per R
+
+// CTAs an SM that the registers are held to: a lane keeps NV R pieces of four.
+constexpr int kDeltaBlocks(int nv, int r) { return nv * r <= 4 ? 4 : nv * r <= 8 ? 3 : 2; }
 
 // One CTA: 32 R rows of one head's state [Dv, Dk] of one sequence.  Row v of
 // the state meets k and q along Dk only, so rows are independent: eight lanes
@@ -67,45 +71,42 @@ constexpr int kDeltaRows = kDeltaThreads / kDeltaLanes;    // state rows of a CT
 // rows.  The kernel is bound by the states' traffic (read once, written
 // once); k, q and v are re-read by the CTAs of a head from L2.
 template <typename TX, typename TS, int NV, int R, bool ALIGNED>
-__global__ void __launch_bounds__(kDeltaThreads) delta_step_kernel(const DeltaStepParams p)
+__global__ void __launch_bounds__(kDeltaThreads, kDeltaBlocks(NV, R)) delta_step_kernel(const DeltaStepParams p)
 {
     __shared__ int64_t warp_sum[kDeltaThreads / 32];
-    const int64_t vt = blockIdx.x % p.v_tiles;
-    const int64_t h = (blockIdx.x / p.v_tiles) % p.Nv;
-    const int64_t b = blockIdx.x / p.v_tiles / p.Nv;
+    // 32-bit indexes (the grid is below 2^31); offsets into tensors are 64-bit
+    const unsigned vt = blockIdx.x % p.v_tiles, bh = blockIdx.x / p.v_tiles;
+    const unsigned h = bh % p.Nv, b = bh / p.Nv;
     const int lane = threadIdx.x % kDeltaLanes;
-    const int64_t v0 = vt * (kDeltaRows * R) + threadIdx.x / kDeltaLanes;
+    const int v0 = static_cast<int>(vt) * (kDeltaRows * R) + threadIdx.x / kDeltaLanes;
+    const int Dk = p.Dk, Dv = p.Dv;
 
     const int64_t slot = p.pool.at(b);
     bool live = slot >= 0 && slot < p.pool.slots;
     const bool past = slot >= p.pool.slots;
 
-    float s[R][NV * 4];
-    const int64_t head = slot * p.s_sn + h * p.s_sh;
+    // this lane's elements of row v0 + 32 r: places j * 32 + lane * 4 and the next three
+    TS* row[R];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int64_t v = v0 + r * kDeltaRows;
+    for (int r = 0; r < R; ++r)
+        row[r] = static_cast<TS*>(p.state) + slot * p.s_sn + h * p.s_sh + (v0 + r * kDeltaRows) * p.s_sv + lane * 4;
+    Pack<TS, 4> raw[R][NV];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int e = (j * kDeltaLanes + lane) * 4;
-            if (live && v < p.Dv && e < p.Dk) {
-                const auto pk = load_pack<TS, 4, ALIGNED>(static_cast<const TS*>(p.state) + head + v * p.s_sv + e,
-                                                          static_cast<int>(p.Dk) - e);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[r][j * 4 + i] = to_f32(pk.e[i]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[r][j * 4 + i] = 0.0f;
-            }
+            const int left = Dk - (j * kDeltaLanes + lane) * 4;
+            raw[r][j] = pack_zero<TS, 4>();
+            if (live && v0 + r * kDeltaRows < Dv && left > 0)
+                raw[r][j] = load_pack<TS, 4, ALIGNED>(row[r] + j * kDeltaLanes * 4, left);
         }
-    }
 
     // the row's first token, and whether an earlier row owns its state
     int64_t begin = b, len = 1;
     bool cut = false;
     if (p.lens) {
         int64_t sum = 0;
-        for (int64_t i = threadIdx.x; i < b; i += kDeltaThreads) {
+        for (unsigned i = threadIdx.x; i < b; i += kDeltaThreads) {
             const int32_t n = p.lens[i];
             sum += n > 0 ? n : 0;
         }
@@ -129,40 +130,41 @@ __global__ void __launch_bounds__(kDeltaThreads) delta_step_kernel(const DeltaSt
     }
     live = live && !dup;
     const int64_t end = begin + len;
+    const bool last = b == p.B - 1;
     if (p.status && vt == 0 && h == 0 && threadIdx.x == 0) {
-        const int bits = ((past || dup) ? 0x4 : 0) | ((cut || (p.lens && b == p.B - 1 && end != p.T)) ? 0x2 : 0);
+        const int bits = ((past || dup) ? 0x4 : 0) | ((cut || (p.lens && last && end != p.T)) ? 0x2 : 0);
         if (bits) atomicOr(p.status, bits);
     }
 
-    const int64_t hk = h / p.rep;
-    TX* const out = static_cast<TX*>(p.out) + h * p.o_sh;
-    if (live) {
+    const unsigned hk = h / p.rep;
+    TX* out = static_cast<TX*>(p.out) + begin * p.o_st + h * p.o_sh + v0;
+    if (live && len > 0) {
+        float s[R][NV * 4];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int i = 0; i < NV * 4; ++i) s[r][i] = to_f32(raw[r][i / 4].e[i % 4]);
+        const TX* kt = static_cast<const TX*>(p.k) + begin * p.k_st + hk * p.k_sh + lane * 4;
+        const TX* qt = static_cast<const TX*>(p.q) + begin * p.q_st + hk * p.q_sh + lane * 4;
+        const TX* vt_ = static_cast<const TX*>(p.v) + begin * p.v_st + h * p.v_sh + v0;
         for (int64_t t = begin; t < end; ++t) {
-            const TX* const kt = static_cast<const TX*>(p.k) + t * p.k_st + hk * p.k_sh;
-            const TX* const qt = static_cast<const TX*>(p.q) + t * p.q_st + hk * p.q_sh;
             float k[NV * 4], q[NV * 4], vv[R];
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
-                const int e = (j * kDeltaLanes + lane) * 4;
-                if (e < p.Dk) {
-                    const int valid = static_cast<int>(p.Dk) - e;
-                    const auto pk = load_pack<TX, 4, ALIGNED>(kt + e, valid);
-                    const auto pq = load_pack<TX, 4, ALIGNED>(qt + e, valid);
+                const int left = Dk - (j * kDeltaLanes + lane) * 4;
+                Pack<TX, 4> pk = pack_zero<TX, 4>(), pq = pk;
+                if (left > 0) {
+                    pk = load_pack<TX, 4, ALIGNED>(kt + j * kDeltaLanes * 4, left);
+                    pq = load_pack<TX, 4, ALIGNED>(qt + j * kDeltaLanes * 4, left);
+                }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        k[j * 4 + i] = to_f32(pk.e[i]);
-                        q[j * 4 + i] = to_f32(pq.e[i]);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) k[j * 4 + i] = q[j * 4 + i] = 0.0f;
+                for (int i = 0; i < 4; ++i) {
+                    k[j * 4 + i] = to_f32(pk.e[i]);
+                    q[j * 4 + i] = to_f32(pq.e[i]);
                 }
             }
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int64_t v = v0 + r * kDeltaRows;
-                vv[r] = v < p.Dv ? to_f32(static_cast<const TX*>(p.v)[t * p.v_st + h * p.v_sh + v]) : 0.0f;
-            }
+            for (int r = 0; r < R; ++r) vv[r] = v0 + r * kDeltaRows < Dv ? to_f32(vt_[r * kDeltaRows]) : 0.0f;
             const int64_t bi = t * p.b_st + h * p.b_sh;
             const float beta = p.beta_f32 ? static_cast<const float*>(p.beta)[bi]
                                           : to_f32(static_cast<const TX*>(p.beta)[bi]);
@@ -191,37 +193,33 @@ __global__ void __launch_bounds__(kDeltaThreads) delta_step_kernel(const DeltaSt
             }
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                const int64_t v = v0 + r * kDeltaRows;
                 const float d = beta * (vv[r] - a * sk[r]);
 #pragma unroll
                 for (int i = 0; i < NV * 4; ++i) s[r][i] = fmaf(a, s[r][i], d * k[i]);
-                if (lane == 0 && v < p.Dv) out[t * p.o_st + v] = from_f32<TX>(p.scale * fmaf(a, sq[r], d * kq));
+                if (lane == 0 && v0 + r * kDeltaRows < Dv)
+                    out[r * kDeltaRows] = from_f32<TX>(p.scale * fmaf(a, sq[r], d * kq));
             }
+            kt += p.k_st;
+            qt += p.q_st;
+            vt_ += p.v_st;
+            out += p.o_st;
         }
-        if (len > 0) {
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int64_t v = v0 + r * kDeltaRows;
+        for (int r = 0; r < R; ++r)
 #pragma unroll
-                for (int j = 0; j < NV; ++j) {
-                    const int e = (j * kDeltaLanes + lane) * 4;
-                    if (v < p.Dv && e < p.Dk)
-                        store_pack<TS, 4, ALIGNED>(static_cast<TS*>(p.state) + head + v * p.s_sv + e, &s[r][j * 4],
-                                                   static_cast<int>(p.Dk) - e);
-                }
+            for (int j = 0; j < NV; ++j) {
+                const int left = Dk - (j * kDeltaLanes + lane) * 4;
+                if (v0 + r * kDeltaRows < Dv && left > 0)
+                    store_pack<TS, 4, ALIGNED>(row[r] + j * kDeltaLanes * 4, &s[r][j * 4], left);
             }
-        }
     }
     // padded rows, and rows behind the last sequence
-    const int64_t zero_from = live ? end : begin;
-    const int64_t zero_to = b == p.B - 1 ? p.T : end;
+    const int64_t zero_from = live ? end : begin, zero_to = last ? p.T : end;
     if (lane == 0)
-        for (int64_t t = zero_from; t < zero_to; ++t)
+        for (int64_t t = zero_from; t < zero_to; ++t, out += p.o_st)
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int64_t v = v0 + r * kDeltaRows;
-                if (v < p.Dv) out[t * p.o_st + v] = from_f32<TX>(0.0f);
-            }
+            for (int r = 0; r < R; ++r)
+                if (v0 + r * kDeltaRows < Dv) out[r * kDeltaRows] = from_f32<TX>(0.0f);
 }
 
 // ---- the diagonal recurrence --------------------------------------------------------------
@@ -232,7 +230,8 @@ struct LinearStepParams {
     void* out;
     int32_t* status;
     PoolIndex pool;
-    int64_t B, D, tiles;
+    int64_t D;
+    uint32_t tiles;
     int64_t x_sb, g_sb, o_sb, s_sn;
 };
 
@@ -243,8 +242,8 @@ constexpr int kLinearStepThreads = 256;
 template <typename TX, typename TG, int V>
 __global__ void __launch_bounds__(kLinearStepThreads) linear_step_kernel(const LinearStepParams p)
 {
-    const int64_t b = blockIdx.x / p.tiles;
-    const int64_t c = ((blockIdx.x % p.tiles) * kLinearStepThreads + threadIdx.x) * V;
+    const unsigned b = blockIdx.x / p.tiles;
+    const int64_t c = (static_cast<int64_t>(blockIdx.x % p.tiles) * kLinearStepThreads + threadIdx.x) * V;
     const int64_t slot = p.pool.at(b);
     const bool in_pool = slot >= 0 && slot < p.pool.slots;
     const bool mine = c < p.D;
