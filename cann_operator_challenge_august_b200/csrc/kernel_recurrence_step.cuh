@@ -57,8 +57,17 @@ constexpr int kDeltaThreads = 256;
 constexpr int kDeltaLanes = 8;                             // lanes that share one state row
 constexpr int kDeltaRows = kDeltaThreads / kDeltaLanes;    // state rows of a CTA per R
 
-// CTAs an SM that the registers are held to: a lane keeps NV R pieces of four.
-constexpr int kDeltaBlocks(int nv, int r) { return nv * r <= 4 ? 4 : nv * r <= 8 ? 3 : 2; }
+// CTAs an SM that the registers are held to, so that nothing spills: a lane keeps
+// NV R pieces of four.
+constexpr int kDeltaBlocks(int nv, int r) { return nv * r <= 4 ? 3 : 2; }
+
+// What a token brings to a lane: its pieces of k and q, the rows' v, beta and g.
+template <typename TX, int NV, int R>
+struct DeltaToken {
+    Pack<TX, 4> k[NV], q[NV];
+    TX v[R];
+    float beta, g;
+};
 
 // One CTA: 32 R rows of one head's state [Dv, Dk] of one sequence.  Row v of
 // the state meets k and q along Dk only, so rows are independent: eight lanes
@@ -80,6 +89,29 @@ __global__ void __launch_bounds__(kDeltaThreads, kDeltaBlocks(NV, R)) delta_step
     const int lane = threadIdx.x % kDeltaLanes;
     const int v0 = static_cast<int>(vt) * (kDeltaRows * R) + threadIdx.x / kDeltaLanes;
     const int Dk = p.Dk, Dv = p.Dv;
+
+    const unsigned hk = h / p.rep;
+    DeltaToken<TX, NV, R> token;
+    auto load_token = [&](int64_t t) {
+        const TX* const kt = static_cast<const TX*>(p.k) + t * p.k_st + hk * p.k_sh + lane * 4;
+        const TX* const qt = static_cast<const TX*>(p.q) + t * p.q_st + hk * p.q_sh + lane * 4;
+        const TX* const vt_ = static_cast<const TX*>(p.v) + t * p.v_st + h * p.v_sh + v0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int left = Dk - (j * kDeltaLanes + lane) * 4;
+            token.k[j] = token.q[j] = pack_zero<TX, 4>();
+            if (left > 0) {
+                token.k[j] = load_pack<TX, 4, ALIGNED>(kt + j * kDeltaLanes * 4, left);
+                token.q[j] = load_pack<TX, 4, ALIGNED>(qt + j * kDeltaLanes * 4, left);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) token.v[r] = v0 + r * kDeltaRows < Dv ? vt_[r * kDeltaRows] : from_f32<TX>(0.0f);
+        const int64_t bi = t * p.b_st + h * p.b_sh;
+        token.beta = p.beta_f32 ? static_cast<const float*>(p.beta)[bi] : to_f32(static_cast<const TX*>(p.beta)[bi]);
+        token.g = p.g ? p.g[t * p.g_st + h * p.g_sh] : 0.0f;
+    };
+    if (!p.lens) load_token(b);
 
     const int64_t slot = p.pool.at(b);
     bool live = slot >= 0 && slot < p.pool.slots;
@@ -136,7 +168,6 @@ __global__ void __launch_bounds__(kDeltaThreads, kDeltaBlocks(NV, R)) delta_step
         if (bits) atomicOr(p.status, bits);
     }
 
-    const unsigned hk = h / p.rep;
     TX* out = static_cast<TX*>(p.out) + begin * p.o_st + h * p.o_sh + v0;
     if (live && len > 0) {
         float s[R][NV * 4];
@@ -144,31 +175,17 @@ __global__ void __launch_bounds__(kDeltaThreads, kDeltaBlocks(NV, R)) delta_step
         for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int i = 0; i < NV * 4; ++i) s[r][i] = to_f32(raw[r][i / 4].e[i % 4]);
-        const TX* kt = static_cast<const TX*>(p.k) + begin * p.k_st + hk * p.k_sh + lane * 4;
-        const TX* qt = static_cast<const TX*>(p.q) + begin * p.q_st + hk * p.q_sh + lane * 4;
-        const TX* vt_ = static_cast<const TX*>(p.v) + begin * p.v_st + h * p.v_sh + v0;
         for (int64_t t = begin; t < end; ++t) {
+            if (p.lens) load_token(t);
             float k[NV * 4], q[NV * 4], vv[R];
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int left = Dk - (j * kDeltaLanes + lane) * 4;
-                Pack<TX, 4> pk = pack_zero<TX, 4>(), pq = pk;
-                if (left > 0) {
-                    pk = load_pack<TX, 4, ALIGNED>(kt + j * kDeltaLanes * 4, left);
-                    pq = load_pack<TX, 4, ALIGNED>(qt + j * kDeltaLanes * 4, left);
-                }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    k[j * 4 + i] = to_f32(pk.e[i]);
-                    q[j * 4 + i] = to_f32(pq.e[i]);
-                }
+            for (int i = 0; i < NV * 4; ++i) {
+                k[i] = to_f32(token.k[i / 4].e[i % 4]);
+                q[i] = to_f32(token.q[i / 4].e[i % 4]);
             }
 #pragma unroll
-            for (int r = 0; r < R; ++r) vv[r] = v0 + r * kDeltaRows < Dv ? to_f32(vt_[r * kDeltaRows]) : 0.0f;
-            const int64_t bi = t * p.b_st + h * p.b_sh;
-            const float beta = p.beta_f32 ? static_cast<const float*>(p.beta)[bi]
-                                          : to_f32(static_cast<const TX*>(p.beta)[bi]);
-            const float a = p.g ? expf(p.g[t * p.g_st + h * p.g_sh]) : 1.0f;
+            for (int r = 0; r < R; ++r) vv[r] = to_f32(token.v[r]);
+            const float beta = token.beta, a = p.g ? expf(token.g) : 1.0f;
 
             float kq = 0.0f, sk[R], sq[R];
 #pragma unroll
@@ -199,9 +216,6 @@ __global__ void __launch_bounds__(kDeltaThreads, kDeltaBlocks(NV, R)) delta_step
                 if (lane == 0 && v0 + r * kDeltaRows < Dv)
                     out[r * kDeltaRows] = from_f32<TX>(p.scale * fmaf(a, sq[r], d * kq));
             }
-            kt += p.k_st;
-            qt += p.q_st;
-            vt_ += p.v_st;
             out += p.o_st;
         }
 #pragma unroll
