@@ -14,7 +14,7 @@ using namespace cgdr::host;
 namespace {
 
 constexpr int64_t kMaxColumns = 16384;
-// Blocks of the backward pass: four for each of the B200's 148 SMs.  A
+// Blocks of the backward pass at most: four for each of the B200's 148 SMs.  A
 // constant, so that the workspace's size and the order of dweight's sum do
 // not depend on the device that is current.
 constexpr int64_t kBackwardBlocks = 592;
@@ -30,6 +30,16 @@ bool pieces_aligned(const cgdrTensor* t, int64_t v)
            (t->ndim < 2 || t->shape[0] <= 1 || t->strides[0] % v == 0);
 }
 
+uint32_t row_bytes(const cgdrTensor* t) { return static_cast<uint32_t>(t->shape[0] > 1 ? t->strides[0] * bytes_of(t->dtype) : 0); }
+
+// The kernels take rows less than 4 GiB apart.
+cgdrStatus check_row_stride(const cgdrTensor* t, const char* name)
+{
+    if (t->shape[0] > 1 && t->strides[0] >= (int64_t(1) << 30))
+        return fail(CGDR_STATUS_UNSUPPORTED, "%s's rows must be less than 2^30 elements apart", name);
+    return CGDR_STATUS_SUCCESS;
+}
+
 // An optional [R, D] tensor of type dt.
 cgdrStatus check_rows(const cgdrTensor* t, int32_t dt, int64_t R, int64_t D, const char* name)
 {
@@ -38,7 +48,8 @@ cgdrStatus check_rows(const cgdrTensor* t, int32_t dt, int64_t R, int64_t D, con
     if ((st = check_rank(t, 2, name))) return st;
     if (t->dtype != dt) return fail(CGDR_STATUS_BAD_DTYPE, "%s has the wrong type", name);
     if (!shape_is(t, {R, D})) return fail(CGDR_STATUS_BAD_SHAPE, "%s must have shape [R, D]", name);
-    return check_inner_contiguous(t, name);
+    if ((st = check_inner_contiguous(t, name))) return st;
+    return check_row_stride(t, name);
 }
 
 cgdrStatus check_x(const cgdrTensor* x, const cgdrTensor* weight, const char* name)
@@ -55,15 +66,17 @@ cgdrStatus check_x(const cgdrTensor* x, const cgdrTensor* weight, const char* na
     if (!shape_is(weight, {D})) return fail(CGDR_STATUS_BAD_SHAPE, "weight must have shape [D]");
     if (D > kMaxColumns)
         return fail(CGDR_STATUS_UNSUPPORTED, "D must be at most %lld", static_cast<long long>(kMaxColumns));
-    if (R >= (int64_t(1) << 31)) return fail(CGDR_STATUS_UNSUPPORTED, "R must fit in 31 bits");
-    if ((st = check_inner_contiguous(x, name))) return st;
+    if (R >= (int64_t(1) << 31) - 4096) return fail(CGDR_STATUS_UNSUPPORTED, "R must be less than 2^31 - 4096");
+    if ((st = check_inner_contiguous(x, name)) || (st = check_row_stride(x, name))) return st;
     return check_inner_contiguous(weight, "weight");
 }
 
 // Calls f.template operator()<TX, V, LPR, NV>() for x's type and row length.
-// Pieces of 16 bytes: the fewest lanes that hold a row in four pieces a lane
-// (`most`; a lane of a longer row has eight, and one piece where a row fits a
-// warp).  Single columns where rows are not made of such pieces.
+// Pieces of 16 bytes, one a lane up to 512 lanes: few registers a lane and many
+// rows in flight (two pieces in half the lanes: 193 against 188 us forwards on
+// 32768 x 4096, 332 against 234 backwards; with 1024 lanes a row's barrier
+// costs more: 270 against 197 us on 16384 x 8192).  Single columns where rows
+// are not made of such pieces.
 template <typename TX, typename F>
 void with_shape(int64_t D, bool pieces, F& f)
 {
@@ -79,10 +92,10 @@ void with_shape(int64_t D, bool pieces, F& f)
     if (n <= 8) f.template operator()<TX, V, 8, 1>();
     else if (n <= 16) f.template operator()<TX, V, 16, 1>();
     else if (n <= 32) f.template operator()<TX, V, 32, 1>();
-    else if (n <= 64) f.template operator()<TX, V, 32, 2>();
-    else if (n <= 128) f.template operator()<TX, V, 64, 2>();
-    else if (n <= 256) f.template operator()<TX, V, 128, 2>();
-    else if (n <= 512) f.template operator()<TX, V, 256, 2>();
+    else if (n <= 64) f.template operator()<TX, V, 64, 1>();
+    else if (n <= 128) f.template operator()<TX, V, 128, 1>();
+    else if (n <= 256) f.template operator()<TX, V, 256, 1>();
+    else if (n <= 512) f.template operator()<TX, V, 512, 1>();
     else if (n <= 1024) f.template operator()<TX, V, 512, 2>();
     else if (n <= 2048) f.template operator()<TX, V, 1024, 2>();
     else if constexpr (V == 4) f.template operator()<TX, V, 1024, 4>();
@@ -116,8 +129,11 @@ struct LaunchBackward {
     template <typename TX, int V, int LPR, int NV>
     void operator()()
     {
+        // as many blocks as are resident together
+        constexpr int64_t kMost = 148 * norm_backward_blocks(LPR);
+        static_assert(kMost <= kBackwardBlocks, "the workspace holds a row of partial sums a block");
         grid = (p.R + norm_rows(LPR) - 1) / norm_rows(LPR);
-        if (grid > kBackwardBlocks) grid = kBackwardBlocks;
+        if (grid > kMost) grid = kMost;
         const unsigned n = static_cast<unsigned>(grid);
         if (p.gate) norm_backward_kernel<TX, V, LPR, NV, true><<<n, norm_threads(LPR), 0, stream>>>(p);
         else norm_backward_kernel<TX, V, LPR, NV, false><<<n, norm_threads(LPR), 0, stream>>>(p);
@@ -180,15 +196,18 @@ cgdrStatus cgdrRmsNorm(const cgdrTensor* x, const cgdrTensor* weight, const cgdr
         p.scale = static_cast<float*>(y_scale->data);
         p.group = static_cast<int32_t>(group);
     }
-    p.x = x->data; p.x_s = x->strides[0];
+    p.x = x->data; p.x_s = row_bytes(x);
     p.w = weight->data; p.w_f32 = weight->dtype == CGDR_DT_FLOAT32;
-    p.y = y->data; p.y_s = y->strides[0];
+    p.y = y->data; p.y_s = row_bytes(y);
     if (present(residual)) {
-        p.residual = residual->data; p.r_s = residual->strides[0];
-        p.z = z->data; p.z_s = z->strides[0];
+        p.residual = residual->data; p.r_s = row_bytes(residual);
+        p.z = z->data; p.z_s = row_bytes(z);
     }
-    if (present(gate)) { p.gate = gate->data; p.a_s = gate->strides[0]; }
-    p.R = R; p.D = D; p.eps = static_cast<float>(eps);
+    if (present(gate)) { p.gate = gate->data; p.a_s = row_bytes(gate); }
+    p.R = static_cast<int32_t>(R);
+    p.D = static_cast<int32_t>(D);
+    p.eps = static_cast<float>(eps);
+    p.inv_d = static_cast<float>(1.0 / static_cast<double>(D));
     const bool pieces = pieces_aligned(x, V) && pieces_aligned(weight, V) && pieces_aligned(residual, V) &&
                         pieces_aligned(gate, V) && pieces_aligned(y, V) && pieces_aligned(z, V);
     with_type(x->dtype, D, pieces, LaunchForward{p, fp8, static_cast<cudaStream_t>(stream)});
@@ -236,14 +255,17 @@ cgdrStatus cgdrRmsNormBackward(const cgdrTensor* z, const cgdrTensor* weight, co
             return fail(CGDR_STATUS_WORKSPACE_TOO_SMALL, "workspace must be 16-byte aligned");
         p.dw = static_cast<float*>(workspace);
     }
-    p.z = z->data; p.z_s = z->strides[0];
+    p.z = z->data; p.z_s = row_bytes(z);
     p.w = weight->data; p.w_f32 = weight->dtype == CGDR_DT_FLOAT32;
-    p.dy = dy->data; p.dy_s = dy->strides[0];
-    if (present(gate)) { p.gate = gate->data; p.a_s = gate->strides[0]; }
-    if (present(dz)) { p.dz = dz->data; p.dz_s = dz->strides[0]; }
-    if (present(dx)) { p.dx = dx->data; p.dx_s = dx->strides[0]; }
-    if (present(dgate)) { p.dgate = dgate->data; p.da_s = dgate->strides[0]; }
-    p.R = R; p.D = D; p.eps = static_cast<float>(eps);
+    p.dy = dy->data; p.dy_s = row_bytes(dy);
+    if (present(gate)) { p.gate = gate->data; p.a_s = row_bytes(gate); }
+    if (present(dz)) { p.dz = dz->data; p.dz_s = row_bytes(dz); }
+    if (present(dx)) { p.dx = dx->data; p.dx_s = row_bytes(dx); }
+    if (present(dgate)) { p.dgate = dgate->data; p.da_s = row_bytes(dgate); }
+    p.R = static_cast<int32_t>(R);
+    p.D = static_cast<int32_t>(D);
+    p.eps = static_cast<float>(eps);
+    p.inv_d = static_cast<float>(1.0 / static_cast<double>(D));
     const int64_t V = 16 / bytes_of(z->dtype);
     bool pieces = pieces_aligned(weight, V);
     for (const cgdrTensor* t : {z, gate, dy, dz, dx, dgate}) pieces = pieces && pieces_aligned(t, V);
