@@ -17,6 +17,14 @@
 // barrier between warps and the copies run on while the CTA joins.  Every sum
 // is taken in a fixed order, so the results are the same on every run.
 //
+// Pace.  CTAs of neighbouring slabs read and write neighbouring 128 bytes of
+// the same rows; once they drift apart, each access opens a DRAM page of its
+// own.  So the CTAs of up to four slabs form one hardware cluster, and none is
+// more than a segment ahead of its neighbours (a barrier without memory order,
+// waited for a segment later): 166 -> 136 us forwards and 303 -> 229 us
+// backwards on 4 x 8192 x 4096.  Only where all CTAs are resident at once: with
+// several waves it cost 10 % (16 x 1024 x 8192).
+//
 // Backwards, the same with u_t = exp(g_{t+1}) dh_{t+1} folded from the right
 // (the factors A are the same), and with h_{t-1} recomputed from the state
 // that the forward pass saved before each 128 tokens.
@@ -51,7 +59,8 @@ struct ScanParams {
     int64_t B, T, D, N;
     int64_t x_sb, x_st, g_sb, g_st, o_sb, o_st, do_sb, do_st, dx_sb, dx_st, dg_sb, dg_st;
     int64_t h0_sn, ht_sn, dht_sn, dh0_sn;
-    int32_t cluster;
+    int32_t cluster;  // CTAs that share a slab's tokens
+    int32_t pace;     // neighbouring slabs in one hardware cluster (1 with cluster > 1)
 };
 
 // The warp's index in a register that the compiler knows to be uniform, so
@@ -123,19 +132,27 @@ __device__ __forceinline__ Vec<V> vec_exp(Vec<V> g)
 
 // What a warp knows of the sequences' borders (cu_seqlens, or 0 and T), as it
 // walks along the tokens 16 at a time.  The nearest border ahead is kept, so
-// cu_seqlens is searched only where one lies in the 16 tokens.
+// they are searched only where one lies in the 16 tokens or behind them, and
+// the first 32 borders stay in a register of each lane.
 struct ScanBorders {
     int64_t first, last;  // tokens [first, last) belong to sequences
     int64_t ahead;
     int64_t sequence;
+    int64_t kept;         // this lane's border among the first 32
     __device__ __forceinline__ ScanBorders(const ScanParams& p, bool reverse)
-        : first(0), last(p.T), ahead(reverse ? INT64_MAX : INT64_MIN), sequence(0)
+        : first(0), last(p.T), ahead(reverse ? INT64_MAX : INT64_MIN), sequence(0), kept(border(p, threadIdx.x % 32))
     {
         if (p.cu) {
             first = p.cu[0];
             const int64_t end = p.cu[p.N];
             last = end < p.T ? end : p.T;
         }
+    }
+    // border i of cu_seqlens, or of 0, T; past the last one none is near
+    static __device__ __forceinline__ int64_t border(const ScanParams& p, int64_t i)
+    {
+        if (!p.cu) return i == 0 ? 0 : i == 1 ? p.T : INT64_MAX;
+        return i <= p.N ? p.cu[i] : INT64_MAX;
     }
     // Bit i: a sequence begins or ends before token t + i, 0 <= i <= 16.  Where
     // there is one, lane i holds the sequence of token t + i afterwards: the
@@ -150,8 +167,8 @@ struct ScanBorders {
         unsigned near = 0xffffffffu;  // distance of the nearest border past the 17 places
         const int64_t n = p.cu ? p.N : 1;
         for (int64_t i0 = 0; i0 <= n; i0 += 32) {
-            const int64_t i = i0 + lane;
-            const int64_t d = i <= n ? (p.cu ? p.cu[i] : i ? p.T : 0) - t : INT64_MAX;
+            const int64_t at = i0 == 0 ? kept : border(p, i0 + lane);
+            const int64_t d = at == INT64_MAX ? at : at - t;
             const bool here = d >= 0 && d <= kScanSteps;
             if (here) bits |= 1u << d;
             const int64_t far = REVERSE ? -d : d - kScanSteps;
@@ -283,6 +300,18 @@ template <int PENDING>
 __device__ __forceinline__ void scan_wait()
 {
     asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
+
+// A CTA's step: waits until the cluster's CTAs have begun the segment before.
+__device__ __forceinline__ void scan_pace(const ScanParams& p, bool first)
+{
+    if (p.pace == 1) return;
+    if (!first) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void scan_pace_end(const ScanParams& p)
+{
+    if (p.pace > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 
 constexpr uint64_t kScanWaitNs = 2000000000ull;
@@ -640,6 +669,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W)
         const int64_t t = first_token(seg);
         const uint32_t borders = seqs.at<false>(p, b, t), dead = seqs.dead(t);
         const bool plain = (borders | dead) == 0;
+        scan_pace(p, seg == 0);
         const bool there = flight.wait(warp, seg);
         const uint8_t *const px = piece(seg), *const pg = px + RX::kBytes;
 
@@ -707,6 +737,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W)
             }
         }
     }
+    scan_pace_end(p);
     if (p.cluster > 1) scan_cluster_sync();  // none leaves while another may still send to it
 }
 
@@ -790,6 +821,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W)
         const bool plain = (borders | dead) == 0;
         const int64_t chunk = t / kScanChunk;
         Vec<V> h = scan_load_state<V>(p.chunk, p.D, b * chunks + chunk, c, mine && chunk < chunks);  // before this CTA's tokens
+        scan_pace(p, k == 0);
         const bool there = flight.wait(warp, k);
         const uint8_t *const px = piece(k), *const pg = px + RX::kBytes, *const pd = pg + RG::kBytes;
         auto get_x = [&](int l) { return vec_of(RX::get(px, l)); };
@@ -896,6 +928,7 @@ __global__ void __launch_bounds__(W * 32, 16 / W)
         }
         fetch(k + kScanStages);
     }
+    scan_pace_end(p);
     if (p.cluster > 1) scan_cluster_sync();
 }
 
