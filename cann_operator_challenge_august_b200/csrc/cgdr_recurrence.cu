@@ -232,15 +232,12 @@ cgdrStatus check_chunks(const cgdrTensor* t, ScanParams* p)
     return CGDR_STATUS_SUCCESS;
 }
 
-// Warps of a CTA; a CTA's tile of a segment is 16 tokens a warp.
-constexpr int kScanW = 8;
-
 // CTAs of a cluster, which share a slab's tokens: doubled while all CTAs still
 // fit on the GPU at once (`resident` CTAs an SM) and have a tile each.
-int32_t scan_cluster(const ScanParams& p, int64_t slabs, int most, int64_t resident)
+int32_t scan_cluster(const ScanParams& p, int64_t slabs, int tile, int most, int64_t resident)
 {
     int32_t c = 1;
-    while (c < most && c * kScanW * kScanSteps < p.T && 2 * c * slabs <= 148 * resident) c *= 2;
+    while (c < most && c * tile < p.T && 2 * c * slabs <= 148 * resident) c *= 2;
     return c;
 }
 
@@ -266,25 +263,25 @@ cgdrStatus scan_map(const cgdrTensor* t, int V, CUtensorMap* map, const char* na
 }
 
 template <typename K>
-cudaError_t launch_scan(K kernel, ScanParams& p, const ScanMapsTma& maps, int V, int smem, int cluster,
+cudaError_t launch_scan(K kernel, ScanParams& p, const ScanMapsTma& maps, int V, int W, int smem, int cluster,
                         cudaStream_t stream)
 {
-    // two CTAs an SM by registers, one where shared memory does not hold two:
+    // 16 warps an SM by registers, fewer where shared memory does not hold them:
     // the ring, the maps of warps and CTAs, and 1 KB of the system's
-    int64_t resident = 2;
-    const int64_t fit = 227 * 1024 / (smem + V * 512 * (kScanW + kScanW / 2 + cluster) + 256 + 1024);
+    int64_t resident = 16 / W;
+    const int64_t fit = 227 * 1024 / (smem + V * 512 * (W + W / 2 + cluster) + 256 + 1024);
     if (resident > fit) resident = fit;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     const int64_t slabs = (p.D + 32 * V - 1) / (32 * V);
-    p.cluster = scan_cluster(p, slabs * p.B, cluster, resident);
+    p.cluster = scan_cluster(p, slabs * p.B, W * kScanSteps, cluster, resident);
     // Neighbouring slabs keep pace where every CTA has a slab of its own and all
     // are resident at once, two an SM.  (With clusters along the tokens it
     // brought nothing, 318 against 327 us forwards on 65536 x 4096; one CTA an
     // SM leaves too few places for clusters of eight, 120 against 162 us on
     // 32768 x 2048 with fp32 gates.)
     p.pace = 1;
-    if (p.cluster == 1 && resident == 2 && slabs * p.B <= 148 * resident)
+    if (p.cluster == 1 && resident >= 2 && slabs * p.B <= 148 * resident)
         while (p.pace < 4 && slabs % (2 * p.pace) == 0) p.pace *= 2;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -293,7 +290,7 @@ cudaError_t launch_scan(K kernel, ScanParams& p, const ScanMapsTma& maps, int V,
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3(static_cast<unsigned>(slabs * p.cluster), static_cast<unsigned>(p.B));
-    cfg.blockDim = dim3(32 * kScanW);
+    cfg.blockDim = dim3(static_cast<unsigned>(32 * W));
     cfg.dynamicSmemBytes = static_cast<size_t>(smem);
     cfg.stream = stream;
     cfg.attrs = &attr;
@@ -317,10 +314,23 @@ struct ScanLaunch {
     template <typename TX, typename TG, int V, bool TMA>
     void go()
     {
-        error = backward ? launch_scan(scan_backward_kernel<TX, TG, V, kScanW, TMA>, p, maps, V,
-                                       scan_backward_smem<TX, TG, V, kScanW>(), kScanBackwardCluster, stream)
-                         : launch_scan(scan_forward_kernel<TX, TG, V, kScanW, TMA>, p, maps, V,
-                                       scan_forward_smem<TX, TG, V, kScanW>(), kScanForwardCluster, stream);
+        // Eight warps a CTA.  Forwards four, where there are too few slabs for a
+        // CTA each (clusters share the tokens) but enough for clusters of eight
+        // to fill the GPU: 300 against 328 us on 65536 x 4096 (64 slabs), but
+        // 225 against 182 us on 65536 x 2048 (32 slabs).  With cu_seqlens eight:
+        // a border holds up a longer segment less often (130 against 159 us for
+        // 16 sequences in 32768 x 2048).
+        const int64_t slabs = (p.D + 32 * V - 1) / (32 * V) * p.B;
+        const bool four = !p.cu && slabs <= 148 && slabs * kScanForwardCluster >= 148 * 3;
+        if (backward)
+            error = launch_scan(scan_backward_kernel<TX, TG, V, 8, TMA>, p, maps, V, 8, scan_backward_smem<TX, TG, V, 8>(),
+                                kScanBackwardCluster, stream);
+        else if (four)
+            error = launch_scan(scan_forward_kernel<TX, TG, V, 4, TMA>, p, maps, V, 4, scan_forward_smem<TX, TG, V, 4>(),
+                                kScanForwardCluster, stream);
+        else
+            error = launch_scan(scan_forward_kernel<TX, TG, V, 8, TMA>, p, maps, V, 8, scan_forward_smem<TX, TG, V, 8>(),
+                                kScanForwardCluster, stream);
     }
     template <typename TX, typename TG>
     void operator()()
