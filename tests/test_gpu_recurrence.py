@@ -105,6 +105,25 @@ def test_scan_long(B, T, D):
     check_scan(B, T, D, BF, BF, seed=5)
 
 
+@pytest.mark.parametrize("B,T,D", [
+    (4, 300, 2560),    # a CTA for each of 160 slabs, clusters of four that keep pace, three segments
+    (3, 300, 3264),    # 153 slabs of an odd count a row: no neighbours to keep pace with
+    (5, 150, 4096),    # more CTAs than the GPU holds at once
+    (1, 1100, 3712),   # 58 slabs: clusters of eight CTAs of four warps
+])
+def test_scan_launch_shapes(B, T, D):
+    """The ways the grid is laid out; a sample of the channels against the definition."""
+    x, g = rand(B, T, D, seed=1, dtype=BF), gates(B, T, D, seed=2, dtype=BF)
+    h0, do, dht = rand(B, D, seed=3), rand(B, T, D, seed=4, dtype=BF), rand(B, D, seed=5)
+    leaves = [t.requires_grad_() for t in (x, g, h0)]
+    o, ht = cg.gated_linear_recurrence(*leaves, output_final_state=True)
+    dx, dg, dh0 = torch.autograd.grad((o, ht), leaves, (do, dht))
+    at = torch.cat([torch.arange(0, D, 61), torch.arange(D - 3, D)]).to(dev())
+    val, err = R.linear_recurrence(x[..., at], g[..., at], h0[..., at], None, do[..., at], dht[..., at])
+    for n, t, kind in (("o", o, BF), ("ht", ht, F32), ("dx", dx, BF), ("dg", dg, BF), ("dh0", dh0, F32)):
+        within(t[..., at], val[n], R.rounded(err[n], val[n], kind), n)
+
+
 def test_scan_strided_views():
     wide = rand(2, 200, 3, 64, seed=1, dtype=BF)
     g = gates(200, 2, 64, seed=2).transpose(0, 1)
@@ -375,6 +394,35 @@ def test_delta_full_batches():
     lens = [(i * 5 + 2) % 4 for i in range(600)]
     t = delta_inputs(lens, 1, 1, 64, 64, BF, F32, 600, seed=2)
     check_delta(t, lens, list(range(599, -1, -1)))
+
+
+def test_delta_float32_beta_and_inference_mode():
+    t = delta_inputs([1] * 3, 2, 4, 64, 64, BF, F32, 5, seed=11)
+    t["beta"] = torch.sigmoid(rand(3, 4, seed=12))
+    with torch.inference_mode():
+        check_delta(t, [1] * 3, [4, 1, 0])
+        x, g, state = rand(3, 64, seed=1), gates(3, 64, seed=2), rand(5, 64, seed=3)
+        assert torch.isfinite(cg.gated_linear_recurrence_step(x, g, state)).all()
+        assert torch.isfinite(cg.gated_linear_recurrence(x[None], g[None])[0]).all()
+
+
+def test_updates_are_seen_by_autograd():
+    """A pool that a graph has saved and a step then changes is refused by the
+    backward pass, as after any in-place operation."""
+    state = rand(3, 64, seed=3).requires_grad_()
+    pool = state * 1.0
+    loss = pool.square().sum()
+    with torch.no_grad():
+        cg.gated_linear_recurrence_step(rand(3, 64, seed=1), gates(3, 64, seed=2), pool)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        loss.backward()
+
+
+def test_second_derivatives_are_refused():
+    x, g = rand(1, 5, 8, seed=1).requires_grad_(), gates(1, 5, 8, seed=2)
+    o, _ = cg.gated_linear_recurrence(x, g)
+    with pytest.raises(RuntimeError, match="once"):
+        torch.autograd.grad(o.sum(), x, create_graph=True)
 
 
 def test_delta_long_sequence():
