@@ -104,21 +104,25 @@ void run_delta(DeltaStepParams& p, cudaStream_t stream)
 template <typename TX, typename TS>
 void dispatch_delta(DeltaStepParams& p, bool aligned, cudaStream_t stream)
 {
-    // Two state rows per lane group once that still leaves two CTAs for each SM.
-    const bool wide = static_cast<int64_t>(p.B) * p.Nv * ((p.Dv + 2 * kDeltaRows - 1) / (2 * kDeltaRows)) >= 296;
+    // Two state rows a lane group where that still gives every SM a CTA: 52
+    // against 61 us for 64 rows of 32 heads of 128 x 128, 4.1 against 5.5 us for
+    // 4, 3.0 against 2.8 us for one (32 heads, 64 CTAs).  Rows of more than 128
+    // take a lane's registers alone: 28 against 32 us for 16 rows of 16 heads of
+    // 256 x 256 with one.
+    const bool wide = static_cast<int64_t>(p.B) * p.Nv * ((p.Dv + 2 * kDeltaRows - 1) / (2 * kDeltaRows)) >= 148;
     const int nv = p.Dk <= 64 ? 2 : p.Dk <= 128 ? 4 : 8;
     if (!aligned) {
         if (nv == 2) run_delta<TX, TS, 2, 1, false>(p, stream);
         else if (nv == 4) run_delta<TX, TS, 4, 1, false>(p, stream);
         else run_delta<TX, TS, 8, 1, false>(p, stream);
+    } else if (nv == 8) {
+        run_delta<TX, TS, 8, 1, true>(p, stream);
     } else if (wide) {
         if (nv == 2) run_delta<TX, TS, 2, 2, true>(p, stream);
-        else if (nv == 4) run_delta<TX, TS, 4, 2, true>(p, stream);
-        else run_delta<TX, TS, 8, 2, true>(p, stream);
+        else run_delta<TX, TS, 4, 2, true>(p, stream);
     } else {
         if (nv == 2) run_delta<TX, TS, 2, 1, true>(p, stream);
-        else if (nv == 4) run_delta<TX, TS, 4, 1, true>(p, stream);
-        else run_delta<TX, TS, 8, 1, true>(p, stream);
+        else run_delta<TX, TS, 4, 1, true>(p, stream);
     }
 }
 
