@@ -102,11 +102,18 @@ __device__ __forceinline__ void row_reduce(float (&v)[N], float (*shared)[32])
         for (int k = 0; k < N; ++k)
             if (threadIdx.x % 32 == 0) shared[k][threadIdx.x / 32] = v[k];
         __syncthreads();
+        // every warp joins the warps' values by shuffles (reading all of them
+        // would be the longer half of a lane's instructions)
+        constexpr int W = LPR / 32;
+        const int lane = threadIdx.x % 32;
 #pragma unroll
         for (int k = 0; k < N; ++k) {
-            v[k] = shared[k][0];
+            v[k] = shared[k][lane % W];
 #pragma unroll
-            for (int i = 1; i < LPR / 32; ++i) v[k] = MAX ? max_nan(v[k], shared[k][i]) : v[k] + shared[k][i];
+            for (int m = W / 2; m > 0; m >>= 1) {
+                const float o = __shfl_xor_sync(~0u, v[k], m);
+                v[k] = MAX ? max_nan(v[k], o) : v[k] + o;
+            }
         }
     }
 }
@@ -145,10 +152,13 @@ __device__ __forceinline__ void norm_store_fp8(uint8_t* to, const float* v)
 // input is read once and every output written once: the kernel is bound by
 // DRAM.  Piece j of lane l holds columns (j LPR + l) V .. + V.  z is kept as it
 // is stored, in its own type, and the weight is read after the row's sum (from
-// L1), so that few registers leave many rows in flight: blocks that walk over
-// the rows with the weight in registers and the next row prefetched were
-// slower (244 against 226 us on 32768 x 4096), and so were two or four rows a
-// lane (1048576 x 128, gated: 204 and 264 against 165 us).
+// L1), so that few registers leave many rows in flight: 183 us on 32768 x 4096
+// bf16 with a residual (5.9 TB/s), 144 us on 1048576 x 128 gated (5.6), 152 us
+// of it in e4m3 (4.4, bound by instructions).  Blocks that walk over the rows
+// with the weight in registers and the next row prefetched were slower when
+// they were tried (244 against 226 us on 32768 x 4096), and so were two or four
+// rows a lane (204 and 264 against 165 us on 1048576 x 128) and twice the
+// pieces in half the lanes (163 against 144 us there).
 template <typename TX, int V, int LPR, int NV, bool FP8>
 __global__ void __launch_bounds__(norm_threads(LPR), norm_forward_blocks(LPR, NV)) norm_forward_kernel(const NormParams p)
 {
@@ -264,8 +274,9 @@ __global__ void __launch_bounds__(norm_threads(LPR), norm_forward_blocks(LPR, NV
 //     dx = r u - z r^3 mean(u z) + dz,   r = (mean(z^2) + eps)^(-1/2)
 // so r is recomputed from z rather than kept.  Blocks walk over the rows; a
 // lane's columns stay the same, so the weight and dweight's share live in
-// registers.  (Prefetching the next row took the registers of half the warps:
-// 310 against 234 us on 32768 x 4096.)  dweight leaves a block once, summed
+// registers: 219 us on 32768 x 4096 bf16 with a residual (4.9 TB/s), 240 us on
+// 1048576 x 128 gated (5.6).  Prefetching the next row took the registers of
+// half the warps (310 against 234 us on 32768 x 4096 when it was tried).  dweight leaves a block once, summed
 // over its rows in a fixed order, and a second kernel adds the blocks.
 template <typename TX, int V, int LPR, int NV, bool GATE>
 __global__ void __launch_bounds__(norm_threads(LPR), norm_backward_blocks(LPR))

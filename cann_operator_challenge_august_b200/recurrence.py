@@ -235,7 +235,7 @@ def gated_linear_recurrence(
     ``[N, D]`` fp32.  With ``cu_seqlens`` (int64 ``[N + 1]`` from 0,
     non-decreasing, B = 1) the sequences are packed along T; an empty one
     keeps its initial state, and rows behind the last one are zero, with zero
-    gradients.  The state is held in fp32.
+    gradients.  Last dimensions are contiguous.  The state is held in fp32.
 
     Differentiable in x, g and initial_state (once).  The gradients are those
     of the recurrence in fp32, recomputed from x, g and one saved state per

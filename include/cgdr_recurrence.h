@@ -75,8 +75,10 @@ cgdrStatus cgdrRecurrentGatedDeltaRule(
  *     chunk_states   [B, ceil(T/128), D]  fp32, contiguous: the state
  *                               before each 128-token chunk (NULL unless a backward
  *                               pass follows)
- * Rows of `out` behind the last sequence are zero.  The state is held in
- * fp32; out is rounded once.  An empty sequence's final state is its initial
+ * T and D are below 2^30, N below 2^16, and rows less than 2^25 elements
+ * apart.  Innermost dimensions are contiguous; rows of 16-byte multiples are
+ * read by TMA, others by smaller copies.  Rows of `out` behind the last
+ * sequence are zero.  The state is held in fp32; out is rounded once.  An empty sequence's final state is its initial
  * state. */
 cgdrStatus cgdrGatedLinearRecurrence(
     const cgdrTensor* x, const cgdrTensor* g, const cgdrTensor* initial_state, const cgdrTensor* cu_seqlens,

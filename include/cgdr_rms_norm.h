@@ -10,9 +10,10 @@
  *
  *     x, residual, gate, z, y   [R, D]  bf16, fp16 or fp32, one type
  *     weight                    [D]     the same type, or fp32
- * with D <= 16384, innermost dimensions contiguous and row strides free.
- * Rows whose address and length are multiples of 16 bytes are read in
- * 16-byte pieces.  Sums are held in fp32; y is rounded once.
+ * with D <= 16384, R < 2^31 - 4096, innermost dimensions contiguous and rows
+ * less than 2^30 elements apart.  Rows whose address and length are multiples
+ * of 16 bytes are read in 16-byte pieces.  Sums are held in fp32; y is rounded
+ * once.
  *
  * Each call checks its arguments (no device work on failure) and enqueues
  * its kernels on `stream`, whose device must be current.

@@ -1,5 +1,5 @@
 """Float64 evaluations of the token-by-token recurrences and the norm --
-TEST INFRASTRUCTURE ONLY (the checker, never the product).
+TEST INFRASTRUCTURE ONLY (a measuring stick, never the product).
 
 Each function takes torch tensors of any type, evaluates the definition in
 float64 on the CPU without intermediate rounding, and returns float64
