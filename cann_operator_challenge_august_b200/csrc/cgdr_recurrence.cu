@@ -302,11 +302,17 @@ cudaError_t launch_scan(K kernel, ScanParams& p, const ScanMapsTma& maps, int V,
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<const ScanParams>(p), maps);
 }
 
-// How the rows are read: by TMA with two channels a lane, by cp.async with two
-// where rows are no multiple of 16 bytes, else one channel a lane.  (Four
-// channels a lane, 256-byte rows of 16-bit types, leave one CTA an SM and were
-// slower: 382 against 302 us forwards on 65536 x 4096.)
+// How the rows are read: by TMA with two channels a lane (or one, below), by
+// cp.async with two where rows are no multiple of 16 bytes, else one channel a
+// lane.  (Four channels a lane, 256-byte rows of 16-bit types, leave one CTA an
+// SM and were slower: 382 against 302 us forwards on 65536 x 4096.)
 enum class ScanPath { kTma, kPairs, kSingle };
+
+// Channels a lane by TMA: two, but one of 16-bit x with fp32 gates, whose ring
+// would leave one CTA an SM (146 against 184 us forwards and 318 against 376 us
+// backwards on 65536 x 1024 with 8 sequences, 160 and 255 against 164 and 262 us
+// on 32768 x 2048 with 16).
+constexpr int scan_channels(int64_t x_bytes, int64_t g_bytes) { return x_bytes == 2 && g_bytes == 4 ? 1 : 2; }
 
 struct ScanLaunch {
     ScanParams& p;
@@ -339,7 +345,7 @@ struct ScanLaunch {
     template <typename TX, typename TG>
     void operator()()
     {
-        if (path == ScanPath::kTma) go<TX, TG, 2, true>();
+        if (path == ScanPath::kTma) go<TX, TG, scan_channels(sizeof(TX), sizeof(TG)), true>();
         else if (path == ScanPath::kPairs) go<TX, TG, 2, false>();
         else go<TX, TG, 1, false>();
     }
@@ -351,11 +357,12 @@ cgdrStatus run_scan(ScanParams& p, const cgdrTensor* x, const cgdrTensor* g, con
     bool pairs = pieces_aligned(x, 2) && pieces_aligned(g, 2) && pieces_aligned(d_out, 2);
     for (const cgdrTensor* t : outs) pairs = pairs && pieces_aligned(t, 2);
     const bool tma = pairs && tma_rows(x) && tma_rows(g) && tma_rows(d_out);
+    const int V = scan_channels(bytes_of(x->dtype), bytes_of(g->dtype));
     ScanMapsTma maps;
     memset(&maps, 0, sizeof(maps));
     cgdrStatus st;
-    if (tma && ((st = scan_map(x, 2, &maps.x, "x")) || (st = scan_map(g, 2, &maps.g, "g")) ||
-                (st = scan_map(d_out, 2, &maps.d_out, "d_out"))))
+    if (tma && ((st = scan_map(x, V, &maps.x, "x")) || (st = scan_map(g, V, &maps.g, "g")) ||
+                (st = scan_map(d_out, V, &maps.d_out, "d_out"))))
         return st;
     ScanLaunch launch{p, maps, tma ? ScanPath::kTma : pairs ? ScanPath::kPairs : ScanPath::kSingle, backward,
                       static_cast<cudaStream_t>(stream)};

@@ -37,8 +37,8 @@
 // What bounds it.  On 4 x 8192 x 4096 bf16 DRAM: 135 us forwards, 229 us
 // backwards, 5.9 TB/s both.  With fewer slabs than SMs the segments' latency:
 // 300 and 500 us on 65536 x 4096 (5.4 TB/s), and on 32768 x 2048 with fp32
-// gates 123 and 195 us (4.4 and 4.8).  A border between sequences holds up the
-// cluster whose warp meets it by 2 to 4 us: 16 of them 165 and 263 us.
+// gates 119 and 197 us (4.5 and 4.8).  A border between sequences holds up the
+// cluster whose warp meets it by 2 to 4 us: 16 of them 160 and 255 us.
 #pragma once
 
 #include <cuda.h>
